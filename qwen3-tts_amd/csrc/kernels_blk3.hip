@@ -130,8 +130,8 @@ __global__ __launch_bounds__(blk3::NTH, 2) void resblock3_bf16_kernel(ResBlock3A
     float *Pm = reinterpret_cast<float *>(smem);                        // [3 units][6][96]: b1 | sn2_a | sn2_ib | b2 | psn_a | psn_ib
     uint4 *Ab = reinterpret_cast<uint4 *>(smem + A_OFF);                // [12][XWB] activated tile, index 54 = the step's first position
     uint4 *Hs = reinterpret_cast<uint4 *>(smem + H_OFF);                // history stores, unit u at [12][6 d_u] from element hoff[u]
-    const unsigned ring_lds = (unsigned)(size_t)(b3_lptr_t)(smem + R_OFF);
-    const unsigned ab_lds = (unsigned)(size_t)(b3_lptr_t)(smem + A_OFF);
+    const unsigned ring_lds = (unsigned)(size_t)(b3_lptr_t)smem + R_OFF;
+    const unsigned ab_lds = (unsigned)(size_t)(b3_lptr_t)smem + A_OFF;
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, h = lane >> 5;

@@ -8,7 +8,7 @@ objs=" kernels.o kernels_bf16.o kernels_bf16_ring.o kernels_blk3.o kernels_enc.o
 for src in ${srcs//,/ }; do
   base=${src%.*}
   extra=""; [ "$base" = kernels_wino ] && extra="-fno-slp-vectorize"
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function $extra $flags -c $src -o /tmp/${base}_$tag.o || exit 1
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops $extra $flags -c $src -o /tmp/${base}_$tag.o || exit 1
   objs=${objs/ $base.o / /tmp/${base}_$tag.o }
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -o ../variants/libhipvoc_$tag.so $objs || exit 1
