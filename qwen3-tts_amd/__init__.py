@@ -8,5 +8,7 @@ from . import hipvoc  # noqa: F401
 from . import wire  # noqa: F401
 from . import voice  # noqa: F401
 from . import encoder  # noqa: F401
+from . import ops  # noqa: F401
 from .encoder import HipSpeechTokenizer  # noqa: F401
 from .hipvoc import HipVocoder, HipVocError, lib_path, load_library  # noqa: F401
+from .ops import HipOps, KvCache  # noqa: F401

@@ -144,6 +144,7 @@ struct Ctx {
     bool wino = true;          // fp32 mode: k = 7 convs of the un-fused residual units by Winograd F(2,7) (HIPVOC_WINO=0: direct)
     bool trim_right = false;   // trans-conv trim policy (metadata transconv_trim_right_only=1): keep L*r samples instead of (L-1)*r
     bool is_encoder = false;   // handle made by hipvoc_enc_load (encoder.inc.cpp): the vocoder entry points refuse it
+    bool is_ops = false;       // handle made by hipvoc_ops_open (ops.inc.cpp): no model; the vocoder and encoder entry points refuse it
     bool bf16 = false;         // HIPVOC_DTYPE_BF16: conv-GEMM operands in bf16, fp32 accumulate, everything else fp32
     bool split3 = false;       // HIPVOC_DTYPE_BF16X3: bf16 = true as well; operands as two bf16 planes, three MFMAs per product
     int dual_out = 1;          // un-fused residual units, SnakeBeta in the producer's epilogue: 0 never, 1 conv7 -> conv1 only
@@ -1599,6 +1600,7 @@ static int decode_host_safe(Ctx *c, const void *codes, const int32_t *n_frames, 
 }
 
 static void enc_release(Ctx *c);      // encoder.inc.cpp
+static int ops_sync_device(Ctx *c);   // ops.inc.cpp
 
 // last failed hipvoc_load / hipvoc_enc_load (no handle to hang the text on)
 static void set_load_error(const char *m) noexcept {
@@ -1719,7 +1721,8 @@ void *hipvoc_load(const char *weights_path, int device_id, int dtype, int unit_f
 // vocoder entry points: not on an encoder handle
 #define DEC(h)                    \
     CTX(h)                        \
-    if (c->is_encoder) { c->err = "this handle is an encoder (hipvoc_enc_load)"; return HIPVOC_E_ARG; }
+    if (c->is_encoder) { c->err = "this handle is an encoder (hipvoc_enc_load)"; return HIPVOC_E_ARG; }  \
+    if (c->is_ops) { c->err = "this handle is an operator handle (hipvoc_ops_open)"; return HIPVOC_E_ARG; }
 
 int hipvoc_max_tokens(void *h) { return h ? ((Ctx *)h)->unit_frames : HIPVOC_E_ARG; }
 int hipvoc_n_codebooks(void *h) { return h ? ((Ctx *)h)->n_q : HIPVOC_E_ARG; }
@@ -1771,6 +1774,7 @@ int hipvoc_decode_units_device_noalloc(void *h, const int64_t *d_codes, int n_un
 
 int hipvoc_sync(void *h) {
     return guarded(h, [&]() -> int {
+        if (h && static_cast<Ctx *>(h)->is_ops) return ops_sync_device(static_cast<Ctx *>(h));
         CTX(h)
         if (c->is_encoder) {
             HIPCHK(hipStreamSynchronize(c->stream));
@@ -1912,12 +1916,17 @@ const char *hipvoc_last_error(void *h) {
 void hipvoc_free(void *h) {
     Ctx *c = (Ctx *)h;
     if (!c) return;
+    int before = c->device;
+    if (c->is_ops) (void)hipGetDevice(&before);      // operator handles leave the caller's current device as it was
     (void)hipSetDevice(c->device);
     (void)hipDeviceSynchronize();
     enc_release(c);
+    const int device = c->device;
     delete c;
+    if (before != device) (void)hipSetDevice(before);
 }
 
 }  // extern "C"
 
 #include "encoder.inc.cpp"
+#include "ops.inc.cpp"

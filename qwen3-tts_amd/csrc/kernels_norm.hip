@@ -1,0 +1,193 @@
+// Root-mean-square norm with the residual's addition (include/hipvoc_ops.h: hipvoc_add_rmsnorm), in the act type or in 8 bits.
+//
+// Mathematics: s = x + r, y = s / sqrt(mean s^2 + eps) * w; 8 bits: y ~ code * (max|y| / TOP) per group of columns.  Everything in 32
+// bits; s is rounded once where it is stored, y once (or to a code).
+// Bound: memory (and, for a few rows, the latency of one load, one reduction and one store).  A row is read once and stays in
+// registers: NV vectors of eight values per thread, TH threads per row; rows of up to 64 * 8 * 4 values are a wave's own, four rows to a
+// workgroup, so the usual reduction is a butterfly without a barrier.
+#include "ops_device.h"
+
+namespace hipvoc {
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ float wave_amax(float v, int width = 64) {
+    for (int o = 1; o < width; o *= 2) v = amax_nan(v, __shfl_xor(v, o));
+    return v;
+}
+
+// OUT == ACT: y in the act type, else codes.  TH threads (64, 256 or 1024) have a row; a workgroup has max(TH, 256) threads.
+template <int ACT, int OUT, int TH, int NV>
+__global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormArgs a) {
+    constexpr int ROWS = TH < 256 ? 256 / TH : 1, NWAVE = TH / 64;
+    typedef typename Store<ACT>::type act_t;
+    __shared__ float sh[2][NWAVE > 1 ? NWAVE : 1];
+    const int t = threadIdx.x % TH, row = blockIdx.x * ROWS + threadIdx.x / TH, vecs = a.cols / 8;
+    if (ROWS > 1 && row >= a.rows) return;                      // a wave's own row: no barrier follows
+    const act_t *x = (const act_t *)a.x + row * a.x_stride, *r = (const act_t *)a.residual + row * a.residual_stride;
+    float s[NV][8], w[NV][8], sq = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int i = v * TH + t;
+        if (i < vecs) {
+            load8<ACT>(x + i * 8, s[v]);
+            load8<ACT>((const act_t *)a.weight + i * 8, w[v]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[v][e] = w[v][e] = 0.f;
+        }
+    }
+    if (a.residual) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int i = v * TH + t;
+            if (i < vecs) {
+                float b[8];
+                load8<ACT>(r + i * 8, b);
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[v][e] += b[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) sq = fmaf(s[v][e], s[v][e], sq);
+    }
+    sq = wave_sum(sq);
+    if constexpr (NWAVE > 1) {
+        if ((t & 63) == 0) sh[0][t >> 6] = sq;
+        __syncthreads();
+        sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < NWAVE; i++) sq += sh[0][i];
+    }
+    const float rs = 1.f / sqrtf(sq / (float)a.cols + a.eps);
+    float top = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int i = v * TH + t;
+        if (a.sum && i < vecs) store8<ACT>((act_t *)a.sum + row * a.sum_stride + i * 8, s[v]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            s[v][e] = s[v][e] * rs * w[v][e];
+            if constexpr (OUT != ACT) top = amax_nan(top, s[v][e]);
+        }
+        if constexpr (OUT == ACT) {
+            if (i < vecs) store8<ACT>((act_t *)a.y + row * a.y_stride + i * 8, s[v]);
+        }
+    }
+    if constexpr (OUT != ACT) {
+        uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
+        if (a.group == 0) {
+            top = wave_amax(top);
+            if constexpr (NWAVE > 1) {
+                if ((t & 63) == 0) sh[1][t >> 6] = top;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < NWAVE; i++) top = amax_nan(top, sh[1][i]);
+            }
+            const float scale = scale8<OUT>(top);
+            if (t == 0) a.scales[row] = scale;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int i = v * TH + t;
+                if (i < vecs) *(u32x2 *)(y + i * 8) = codes8<OUT>(s[v], scale);
+            }
+        } else {
+            // a group is 4, 8 or 16 neighbouring lanes of one vector index (TH is a multiple of 16)
+            const int lanes = a.group / 8;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int i = v * TH + t;
+                float g = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) g = amax_nan(g, s[v][e]);
+                const float scale = scale8<OUT>(wave_amax(g, lanes));
+                if (i < vecs) {
+                    *(u32x2 *)(y + i * 8) = codes8<OUT>(s[v], scale);
+                    if (i % lanes == 0) a.scales[(int64_t)row * (a.cols / a.group) + i / lanes] = scale;
+                }
+            }
+        }
+    }
+}
+
+// Any length and alignment: a workgroup per row, one value at a time.  s is made anew in every pass, and the stored sum may be x or the
+// residual: it is written last, behind a barrier where another thread may still read its place.
+template <int ACT, int OUT>
+__global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(NormArgs a) {
+    typedef typename Store<ACT>::type act_t;
+    __shared__ float sh[4];
+    const int t = threadIdx.x, row = blockIdx.x;
+    const act_t *x = (const act_t *)a.x + row * a.x_stride, *r = (const act_t *)a.residual + row * a.residual_stride;
+    auto s_of = [&](int i) { return (float)x[i] + (a.residual ? (float)r[i] : 0.f); };
+    float sq = 0.f;
+    for (int i = t; i < a.cols; i += 256) {
+        const float s = s_of(i);
+        sq = fmaf(s, s, sq);
+    }
+    sq = wave_sum(sq);
+    if ((t & 63) == 0) sh[t >> 6] = sq;
+    __syncthreads();
+    const float rs = 1.f / sqrtf((sh[0] + sh[1] + sh[2] + sh[3]) / (float)a.cols + a.eps);
+    auto y_of = [&](int i) { return s_of(i) * rs * (float)((const act_t *)a.weight)[i]; };
+    if constexpr (OUT == ACT) {
+        for (int i = t; i < a.cols; i += 256) {
+            const float s = s_of(i);
+            store1<ACT>(a.y, row * a.y_stride + i, s * rs * (float)((const act_t *)a.weight)[i]);
+            if (a.sum) store1<ACT>(a.sum, row * a.sum_stride + i, s);
+        }
+    } else {
+        uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
+        const int n = a.group ? a.group : a.cols, groups = a.cols / n, lane = t & 63;
+        // a group per wave; the whole row: all four waves find the same maximum over all of it, and each codes a quarter
+        const bool whole = a.group == 0;
+        for (int g = whole ? 0 : t >> 6; g < groups; g += 4) {
+            float top = 0.f;
+            for (int i = lane; i < n; i += 64) top = amax_nan(top, y_of(g * n + i));
+            const float scale = scale8<OUT>(wave_amax(top));
+            if (lane == 0 && (!whole || t == 0)) a.scales[(int64_t)row * groups + g] = scale;
+            for (int i = whole ? t : lane; i < n; i += whole ? 256 : 64) y[g * n + i] = code1<OUT>(y_of(g * n + i), scale);
+        }
+        __syncthreads();
+        if (a.sum)
+            for (int i = t; i < a.cols; i += 256) store1<ACT>(a.sum, row * a.sum_stride + i, s_of(i));
+    }
+}
+
+template <int ACT, int OUT, int TH, int NV> static void norm_go(const NormArgs &a, hipStream_t s) {
+    constexpr int ROWS = TH < 256 ? 256 / TH : 1;
+    add_rmsnorm_kernel<ACT, OUT, TH, NV><<<(a.rows + ROWS - 1) / ROWS, TH < 256 ? 256 : TH, 0, s>>>(a);
+}
+template <int ACT, int OUT> static hipError_t norm_out(const NormArgs &a, hipStream_t s) {
+    constexpr int A = ACT == HIPVOC_T_F32 ? 4 : 2;
+    auto odd = [](const void *p, int64_t stride, int size) { return (((uintptr_t)p) | (uint64_t)(stride * size)) & 15; };
+    bool any = a.cols % 8 || odd(a.x, a.x_stride, A) || odd(a.weight, 0, A) || (a.residual && odd(a.residual, a.residual_stride, A)) ||
+               (a.sum && odd(a.sum, a.sum_stride, A));
+    any = any || (OUT == ACT ? odd(a.y, a.y_stride, A) != 0 : ((((uintptr_t)a.y) | (uint64_t)a.y_stride) & 7) != 0);
+    const int vecs = a.cols / 8;
+    if (any || vecs > 4096) add_rmsnorm_any_kernel<ACT, OUT><<<a.rows, 256, 0, s>>>(a);
+    else if (vecs <= 64) norm_go<ACT, OUT, 64, 1>(a, s);
+    else if (vecs <= 128) norm_go<ACT, OUT, 64, 2>(a, s);
+    else if (vecs <= 256) norm_go<ACT, OUT, 64, 4>(a, s);
+    else if (vecs <= 512) norm_go<ACT, OUT, 256, 2>(a, s);
+    else if (vecs <= 1024) norm_go<ACT, OUT, 256, 4>(a, s);
+    else norm_go<ACT, OUT, 1024, 4>(a, s);
+    return hipGetLastError();
+}
+template <int ACT> static hipError_t norm_act(const NormArgs &a, hipStream_t s) {
+    if (a.out_dtype == HIPVOC_T_INT8) return norm_out<ACT, HIPVOC_T_INT8>(a, s);
+    if (a.out_dtype == HIPVOC_T_E4M3) return norm_out<ACT, HIPVOC_T_E4M3>(a, s);
+    return norm_out<ACT, ACT>(a, s);
+}
+hipError_t launch_add_rmsnorm(const NormArgs &a, hipStream_t s) {
+    if (a.dtype == HIPVOC_T_F32) return norm_act<HIPVOC_T_F32>(a, s);
+    if (a.dtype == HIPVOC_T_F16) return norm_act<HIPVOC_T_F16>(a, s);
+    return norm_act<HIPVOC_T_BF16>(a, s);
+}
+
+}  // namespace hipvoc
