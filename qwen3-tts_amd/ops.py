@@ -10,7 +10,6 @@ There is NO fallback: if the shared library is missing or no HIP device is prese
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Optional, Tuple
 
 from .hipvoc import HipVocError, load_library
@@ -55,33 +54,28 @@ def _lib():
     return L
 
 
-def _torch():
-    import torch
-    return torch
+torch = None
+_types = {}                     # torch dtype -> HIPVOC_T_*
 
 
-_types = {}
-
-
-def _type(t) -> int:
-    if not _types:
-        torch = _torch()
-        _types.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.int8: T_INT8, torch.float8_e4m3fn: T_E4M3})
-    code = _types.get(t.dtype, -1)
-    if code < 0:
-        raise HipVocError(-1, f"unsupported dtype {t.dtype}")
-    return code
+def _bind_torch():
+    """The rest of the package needs no torch: it is imported when the first cache or handle is made."""
+    global torch
+    if torch is None:
+        import torch as module
+        _types.update({module.float32: T_F32, module.float16: T_F16, module.bfloat16: T_BF16, module.int8: T_INT8, module.float8_e4m3fn: T_E4M3})
+        torch = module
 
 
 def _refuse(msg: str):
     raise HipVocError(-1, msg)
 
 
-def _int32(**values):
-    """The C entry points take 32-bit integers; ctypes would wrap a larger one silently."""
-    for name, v in values.items():
-        if not -(1 << 31) <= v < 1 << 31:
-            _refuse(f"{name} = {v} does not fit 32 bits")
+def _type(t) -> int:
+    code = _types.get(t.dtype, -1)
+    if code < 0:
+        _refuse(f"unsupported dtype {t.dtype}")
+    return code
 
 
 class KvCache:
@@ -89,6 +83,7 @@ class KvCache:
     k_scale, v_scale [n_pages, kv_heads, page] float32 for int8 / float8_e4m3fn caches."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        _bind_torch()
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             _refuse("k and v must be [n_pages, kv_heads, page, head_dim], alike in shape, type and device")
         n, heads, page, hd = k.shape
@@ -113,11 +108,11 @@ class HipOps:
     """The operators of one token step on one MI355X."""
 
     def __init__(self, handle, lib, device: int):
-        torch = _torch()
+        _bind_torch()
         self._h = handle
         self._L = lib
         self.device = torch.device("cuda", device)
-        self._stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+        self._index = device
 
     @classmethod
     def open(cls, device: int = 0) -> "HipOps":
@@ -138,81 +133,115 @@ class HipOps:
         except Exception:
             pass
 
-    def _check(self, rc: int):
-        if rc != 0:
-            raise HipVocError(rc, self._L.hipvoc_last_error(self._h).decode() if self._h else "the handle is closed")
+    def _failed(self, rc: int):
+        raise HipVocError(rc, self._L.hipvoc_last_error(self._h).decode() if self._h else "the handle is closed")
 
     @property
     def stream(self) -> int:
         """torch's current stream of the handle's device, where the calls are enqueued."""
-        if self._stream is not None:
-            return self._stream(self.device.index)
-        return _torch().cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def sync(self):
         """Waits for the current stream and raises what the device found wrong since the last time."""
-        self._check(self._L.hipvoc_ops_sync(self._h, self.stream))
+        rc = self._L.hipvoc_ops_sync(self._h, self.stream)
+        if rc:
+            self._failed(rc)
+
+    # ---- what a call looks at in its tensors (a step makes these calls per layer: each attribute is asked for once) -----
+    def _elsewhere(self, name, t):
+        _refuse(f"{name} is on {t.device}, the handle on {self.device}")
+
+    def _here(self, name, t):
+        if t is not None and t.device != self.device:
+            self._elsewhere(name, t)
+
+    def _ints(self, name, t, n):
+        """Address of a contiguous int32 vector of n values."""
+        if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+            _refuse(f"{name} must be a contiguous int32 vector of {n}")
+        if t.device != self.device:
+            self._elsewhere(name, t)
+        return t.data_ptr()
+
+    def _table(self, t):
+        """(address, stride, width, rows) of a page table."""
+        shape = t.shape
+        if t.dtype != torch.int32 or len(shape) != 2:
+            _refuse("table must be int32 [seqs, pages]")
+        stride = t.stride()
+        if shape[1] > 1 and stride[1] != 1:
+            _refuse("table must have contiguous rows")
+        if t.device != self.device:
+            self._elsewhere("table", t)
+        return t.data_ptr(), stride[0], shape[1], shape[0]
+
+    def _heads(self, name, t, heads, hd):
+        """(rows, row stride) of [rows, heads, head_dim] with contiguous rows."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != hd or stride[2] != 1 or (heads > 1 and stride[1] != hd):
+            _refuse(f"{name} must be [rows, {heads}, {hd}] with contiguous rows")
+        if t.device != self.device:
+            self._elsewhere(name, t)
+        rows = shape[0]
+        return rows, stride[0] if rows > 1 else heads * hd
+
+    def _matrix(self, name, t):
+        """(rows, columns, row stride) of a matrix with contiguous rows."""
+        shape = t.shape
+        if len(shape) != 2:
+            _refuse(f"{name} must be a matrix")
+        rows, cols = shape
+        stride = t.stride()
+        if stride[1] != 1 and cols > 1:
+            _refuse(f"{name} must have contiguous rows")
+        if t.device != self.device:
+            self._elsewhere(name, t)
+        return rows, cols, stride[0] if rows > 1 else cols
 
     # ---- the paged cache -----------------------------------------------------------------
     def kv_cache(self, k, v, k_scale=None, v_scale=None) -> KvCache:
-        cache = KvCache(k, v, k_scale, v_scale)
-        self._here(k)
-        return cache
-
-    def _here(self, *tensors):
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                _refuse(f"a tensor is on {t.device}, the handle on {self.device}")
-
-    def _ints(self, name, t, dims):
-        if t.dtype != _torch().int32 or t.dim() != dims or (t.numel() > 0 and t.stride(-1) != 1):
-            _refuse(f"{name} must be int32 with {dims} dimension(s), the last contiguous")
-        if t.device != self.device:
-            _refuse(f"{name} is on {t.device}, the handle on {self.device}")
-        return t.data_ptr()
+        self._here("k", k)
+        return KvCache(k, v, k_scale, v_scale)
 
     def _rows(self, table, cu, first):
-        n = table.shape[0]
-        r = _Rows(self._ints("table", table, 2), self._ints("cu", cu, 1), self._ints("first", first, 1), table.stride(0), table.shape[1], n)
-        if cu.shape[0] != n + 1 or first.shape[0] != n:
-            _refuse("cu must have one entry more than table has rows, first as many")
-        return r
-
-    def _heads(self, name, t, heads, hd):
-        """Row stride of [rows, heads, head_dim] with contiguous rows."""
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or (t.numel() > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd))):
-            _refuse(f"{name} must be [rows, {heads}, {hd}] with contiguous rows")
-        if t.device != self.device:
-            _refuse(f"{name} is on {t.device}, the handle on {self.device}")
-        return t.stride(0) if t.shape[0] > 1 else heads * hd
+        tp, stride, width, n = self._table(table)
+        return _Rows(tp, self._ints("cu", cu, n + 1), self._ints("first", first, n), stride, width, n)
 
     def kv_write(self, cache: KvCache, k, v, table, cu, first):
         """k, v [rows, kv_heads, head_dim]: rows cu[b] .. cu[b+1] go to positions first[b] ... of sequence b (pages table[b])."""
-        ks, vs = self._heads("k", k, cache.kv_heads, cache.head_dim), self._heads("v", v, cache.kv_heads, cache.head_dim)
-        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+        if cache.device != self.device:
+            self._elsewhere("the cache", cache)
+        n, ks = self._heads("k", k, cache.kv_heads, cache.head_dim)
+        nv, vs = self._heads("v", v, cache.kv_heads, cache.head_dim)
+        if n != nv or k.dtype != v.dtype:
             _refuse("k and v must be alike")
-        self._here(cache.k)
         r = self._rows(table, cu, first)
-        self._check(self._L.hipvoc_kv_write(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), k.shape[0], self.stream))
+        rc = self._L.hipvoc_kv_write(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), n, self.stream)
+        if rc:
+            self._failed(rc)
 
     def kv_read(self, cache: KvCache, table, cu, first, n_rows: int, dtype=None, out: Optional[Tuple] = None):
         """The inverse: (k, v) [n_rows, kv_heads, head_dim] in `dtype` (default: the cache's own), or into the two tensors of `out`;
         rows at or behind cu[-1] are left as they were."""
-        torch = _torch()
-        _int32(n_rows=n_rows)
-        if n_rows < 0:
-            _refuse(f"n_rows {n_rows} is negative")
+        if cache.device != self.device:
+            self._elsewhere("the cache", cache)
+        if not 0 <= n_rows < 1 << 31:
+            _refuse(f"n_rows {n_rows} is negative or does not fit 32 bits")
+        heads, hd = cache.kv_heads, cache.head_dim
         if out is None:
-            shape = (n_rows, cache.kv_heads, cache.head_dim)
-            dtype = dtype or cache.k.dtype
-            out = (torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device))
-        k, v = out
-        ks, vs = self._heads("k", k, cache.kv_heads, cache.head_dim), self._heads("v", v, cache.kv_heads, cache.head_dim)
-        if k.shape[0] < n_rows or v.shape[0] < n_rows or k.dtype != v.dtype:
-            _refuse("out must be two tensors of n_rows rows, alike in type")
-        self._here(cache.k)
+            k = torch.empty((n_rows, heads, hd), dtype=dtype or cache.k.dtype, device=self.device)
+            v = torch.empty_like(k)
+            ks = vs = heads * hd
+        else:
+            k, v = out
+            n, ks = self._heads("k", k, heads, hd)
+            nv, vs = self._heads("v", v, heads, hd)
+            if n < n_rows or nv < n_rows or k.dtype != v.dtype:
+                _refuse("out must be two tensors of n_rows rows, alike in type")
         r = self._rows(table, cu, first)
-        self._check(self._L.hipvoc_kv_read(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), n_rows, self.stream))
+        rc = self._L.hipvoc_kv_read(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), n_rows, self.stream)
+        if rc:
+            self._failed(rc)
         return k, v
 
     # ---- attention of one new token ------------------------------------------------------
@@ -220,94 +249,107 @@ class HipOps:
                   lse: bool = False, out=None):
         """q [seqs, heads, head_dim] over the lens[b] tokens of each sequence -> out like q; with lse=True also the log of the
         softmax's sum [seqs, heads] float32.  max_len: a bound on lens the host knows (default: all the table's pages hold)."""
-        torch = _torch()
-        n, heads = q.shape[0], q.shape[1]
-        qs = self._heads("q", q, heads, cache.head_dim)
-        tp, lp = self._ints("table", table, 2), self._ints("lens", lens, 1)
-        if table.shape[0] != n or lens.shape[0] != n:
-            _refuse("table and lens must have a row per sequence")
-        self._here(cache.k)
-        width = table.shape[1]
+        if cache.device != self.device:
+            self._elsewhere("the cache", cache)
+        hd, heads = cache.head_dim, q.shape[1]
+        n, qs = self._heads("q", q, heads, hd)
+        tp, stride, width, nt = self._table(table)
+        if nt != n:
+            _refuse("table must have a row per sequence")
+        lp = self._ints("lens", lens, n)
         if max_len is None:
             max_len = width * cache.page
-        _int32(window=window, max_len=max_len)
+        if not (0 <= max_len < 1 << 31 and 0 <= window < 1 << 31):
+            _refuse(f"max_len {max_len} or window {window} is negative or does not fit 32 bits")
         if out is None:
-            out = torch.empty((n, heads, cache.head_dim), dtype=q.dtype, device=self.device)
-        os_ = self._heads("out", out, heads, cache.head_dim)
-        if out.shape[0] != n or out.dtype != q.dtype:
-            _refuse("out must be like q")
-        sums = torch.empty((n, heads), dtype=torch.float32, device=self.device) if lse else None
+            out = torch.empty_like(q)
+            os_ = heads * hd
+        else:
+            no, os_ = self._heads("out", out, heads, hd)
+            if no != n or out.dtype != q.dtype:
+                _refuse("out must be like q")
+        sums = q.new_empty((n, heads), dtype=torch.float32) if lse else None
         need = self._L.hipvoc_attention_workspace(cache._p, heads, n, max_len, window)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._check(self._L.hipvoc_attention(
-            self._h, cache._p, q.data_ptr(), qs, out.data_ptr(), os_, sums.data_ptr() if lse else None, _type(q), heads, tp, table.stride(0), width, lp, n,
-            max_len, window, 1.0 / math.sqrt(cache.head_dim) if scale is None else scale, ws.data_ptr() if need else None, need, self.stream))
+        ws = lens.new_empty(need // 4) if need else None
+        rc = self._L.hipvoc_attention(
+            self._h, cache._p, q.data_ptr(), qs, out.data_ptr(), os_, sums.data_ptr() if lse else None, _type(q), heads, tp, stride, width, lp, n,
+            max_len, window, hd ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need, self.stream)
+        if rc:
+            self._failed(rc)
         return (out, sums) if lse else out
 
     # ---- norm ----------------------------------------------------------------------------
-    def _matrix(self, name, t, rows, cols):
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.numel() > 0 and t.stride(1) != 1):
-            _refuse(f"{name} must be [{rows}, {cols}] with contiguous rows")
-        if t.device != self.device:
-            _refuse(f"{name} is on {t.device}, the handle on {self.device}")
-        return t.stride(0) if rows > 1 else cols
-
     def add_rmsnorm(self, x, weight, residual=None, eps: float = 1e-6, quant: Optional[str] = None, group: int = 0):
         """x [rows, cols] (+ residual) -> (sum, y), or with quant "int8" / "e4m3" (sum, codes, scales [rows, cols / group]; group 0:
         one scale per row).  sum is None without a residual."""
-        torch = _torch()
-        if x.dim() != 2:
-            _refuse("x must be [rows, cols]")
-        rows, cols = x.shape
-        xs = self._matrix("x", x, rows, cols)
-        if weight.dtype != x.dtype or weight.dim() != 1 or weight.shape[0] != cols or not weight.is_contiguous():
+        rows, cols, xs = self._matrix("x", x)
+        act = x.dtype
+        t = _type(x)
+        if weight.dtype != act or weight.shape != (cols,) or not weight.is_contiguous():
             _refuse("weight must be a contiguous [cols] of x's type")
-        self._here(weight)
-        rs, total = 0, None
+        if weight.device != self.device:
+            self._elsewhere("weight", weight)
+        rs, rp, total, sp = 0, None, None, None
         if residual is not None:
-            rs = self._matrix("residual", residual, rows, cols)
-            if residual.dtype != x.dtype:
-                _refuse("residual must have x's type")
-            total = torch.empty((rows, cols), dtype=x.dtype, device=self.device)
+            rr, rc, rs = self._matrix("residual", residual)
+            if residual.dtype != act or rr != rows or rc != cols:
+                _refuse("residual must have x's type and shape")
+            total = torch.empty_like(x)
+            rp, sp = residual.data_ptr(), total.data_ptr()
         if quant is None:
-            y, scales, ot = torch.empty((rows, cols), dtype=x.dtype, device=self.device), None, _type(x)
-        elif quant in ("int8", "e4m3"):
-            _int32(group=group)
+            y, scales, ot, cp = torch.empty_like(x), None, t, None
+        elif quant == "int8" or quant == "e4m3":
+            if group and (group not in (32, 64, 128) or cols % group):
+                _refuse(f"group {group} must be 0, or 32, 64 or 128 and a divisor of cols {cols}")
             ot = T_INT8 if quant == "int8" else T_E4M3
-            y = torch.empty((rows, cols), dtype=torch.int8 if quant == "int8" else torch.float8_e4m3fn, device=self.device)
-            scales = torch.empty((rows, cols // group if group > 0 else 1), dtype=torch.float32, device=self.device)
+            y = torch.empty_like(x, dtype=torch.int8 if ot == T_INT8 else torch.float8_e4m3fn)
+            scales = x.new_empty((rows, cols // group if group else 1), dtype=torch.float32)
+            cp = scales.data_ptr()
         else:
             _refuse("quant must be None, 'int8' or 'e4m3'")
-        self._check(self._L.hipvoc_add_rmsnorm(
-            self._h, x.data_ptr(), xs, None if residual is None else residual.data_ptr(), rs, weight.data_ptr(), None if total is None else total.data_ptr(),
-            cols, y.data_ptr(), cols, None if scales is None else scales.data_ptr(), _type(x), ot, group, eps, rows, cols, self.stream))
+        rc = self._L.hipvoc_add_rmsnorm(self._h, x.data_ptr(), xs, rp, rs, weight.data_ptr(), sp, cols, y.data_ptr(), cols, cp, t, ot, group, eps, rows, cols,
+                                        self.stream)
+        if rc:
+            self._failed(rc)
         return (total, y) if quant is None else (total, y, scales)
 
     # ---- 4-bit products ------------------------------------------------------------------
     def q4_matvec(self, codes, scales, x, mins=None, x_scale=None, dtype=None):
         """x [rows, n_in] times the 4-bit weights codes [n_out, n_in / 2] uint8, scales (mins) [n_out, n_in / group] float16 ->
         [rows, n_out].  int8 rows: x_scale [rows, n_in / group] or [rows, 1] float32, and `dtype` of the result (default float32)."""
-        torch = _torch()
-        if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or scales.dim() != 2 or x.dim() != 2:
-            _refuse("codes must be a contiguous uint8 [n_out, n_in / 2], scales [n_out, n_in / group], x [rows, n_in]")
-        n_out, n_in, rows = codes.shape[0], codes.shape[1] * 2, x.shape[0]
-        groups = scales.shape[1]
-        for t in (scales, mins):
-            if t is not None and (t.dtype != torch.float16 or tuple(t.shape) != (n_out, groups) or not t.is_contiguous()):
-                _refuse("scales and mins must be contiguous float16 [n_out, n_in / group]")
-        if groups < 1 or n_in % groups:
-            _refuse("scales must have a column per group of n_in")
-        self._here(codes, scales, mins, x_scale)
-        xs = self._matrix("x", x, rows, n_in)
+        cs, ss = codes.shape, scales.shape
+        if len(cs) != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
+            _refuse("codes must be a contiguous uint8 [n_out, n_in / 2]")
+        n_out, n_in = cs[0], cs[1] * 2
+        if len(ss) != 2 or ss[0] != n_out or scales.dtype != torch.float16 or not scales.is_contiguous() or ss[1] < 1 or n_in % ss[1]:
+            _refuse("scales must be a contiguous float16 [n_out, n_in / group]")
+        here, mp, xp = self.device, None, None
+        if mins is not None:
+            if mins.dtype != torch.float16 or mins.shape != ss or not mins.is_contiguous():
+                _refuse("mins must be like scales")
+            if mins.device != here:
+                self._elsewhere("mins", mins)
+            mp = mins.data_ptr()
+        if codes.device != here or scales.device != here:
+            self._elsewhere("codes or scales", codes if codes.device != here else scales)
+        rows, cols, xs = self._matrix("x", x)
+        if cols != n_in:
+            _refuse(f"x must have {n_in} columns")
         xt, x_groups = _type(x), 0
         if xt == T_INT8:
             if x_scale is None or x_scale.dtype != torch.float32 or x_scale.dim() != 2 or x_scale.shape[0] != rows or not x_scale.is_contiguous():
                 _refuse("int8 rows need x_scale, a contiguous float32 [rows, n_in / group] or [rows, 1]")
-            x_groups = x_scale.shape[1]
+            if x_scale.device != here:
+                self._elsewhere("x_scale", x_scale)
+            x_groups, xp = x_scale.shape[1], x_scale.data_ptr()
+            out = dtype or torch.float32
         elif x_scale is not None:
             _refuse("only int8 rows have scales")
-        y = torch.empty((rows, n_out), dtype=dtype or (torch.float32 if xt == T_INT8 else x.dtype), device=self.device)
-        self._check(self._L.hipvoc_q4_matvec(
-            self._h, codes.data_ptr(), scales.data_ptr(), None if mins is None else mins.data_ptr(), n_out, n_in, n_in // groups, x.data_ptr(), xs, xt,
-            None if x_scale is None else x_scale.data_ptr(), x_groups, y.data_ptr(), n_out, _type(y), rows, self.stream))
+        else:
+            out = dtype or x.dtype
+        y = x.new_empty((rows, n_out), dtype=out)
+        rc = self._L.hipvoc_q4_matvec(self._h, codes.data_ptr(), scales.data_ptr(), mp, n_out, n_in, n_in // ss[1], x.data_ptr(), xs, xt, xp, x_groups,
+                                      y.data_ptr(), n_out, _type(y), rows, self.stream)
+        if rc:
+            self._failed(rc)
         return y
