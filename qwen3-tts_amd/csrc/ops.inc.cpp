@@ -142,7 +142,10 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
 
 size_t hipvoc_attention_workspace(const hipvoc_kv_cache *cache, int n_heads, int n_seqs, int max_len, int window) {
     if (!cache || cache->kv_heads < 1 || n_heads < 1 || n_seqs < 1 || max_len < 1 || window < 0) return 0;
-    return attention_plan(cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window).bytes;
+    // the act type is not asked for: what either kernel needs
+    const bool coded = cache->dtype == HIPVOC_T_INT8 || cache->dtype == HIPVOC_T_E4M3;
+    return std::max(attention_plan(HIPVOC_T_F32, coded, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window).bytes,
+                    attention_plan(HIPVOC_T_BF16, coded, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window).bytes);
 }
 
 int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64_t q_stride, void *out, int64_t out_stride, float *lse, int dtype,
@@ -155,7 +158,7 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
         if (!c->err.empty()) return HIPVOC_E_ARG;
         const int rc = ops_stream(c, stream);
         if (rc || n_seqs == 0) return rc;
-        const AttnPlan p = attention_plan(cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
+        const AttnPlan p = attention_plan(dtype, cache->dtype != dtype, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
         AttnArgs a = {};
         a.page_shift = __builtin_ctz((unsigned)cache->page);
         a.c = *cache;
@@ -175,9 +178,11 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
         a.max_len = max_len;
         a.window = window;
         a.scale_log2 = scale * 1.44269504088896340736f;
-        a.chunk = p.chunk;
-        a.n_chunks = p.n_chunks;
+        a.heads = p.heads;
+        a.workers = p.workers;
+        a.least = p.least;
         a.part = (float *)workspace;
+        a.before = p.workers ? (int64_t *)((char *)workspace + p.bytes) - (n_seqs + 1) : nullptr;
         a.err = c->d_err;
         return ops_launched(c, "hipvoc_attention", launch_attention_decode(a, (hipStream_t)stream));
     });

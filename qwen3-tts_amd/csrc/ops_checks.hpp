@@ -35,7 +35,7 @@ static inline std::string check_cache(const hipvoc_kv_cache *k, int dtype) {
     if (!coded && (k->k_scale || k->v_scale)) return "only an 8-bit cache has scales";
     if (k->head_dim != 64 && k->head_dim != 128) return ops_say("head_dim must be 64 or 128, not %d", k->head_dim);
     if (k->page < 8 || k->page > 1024 || (k->page & (k->page - 1))) return ops_say("page must be a power of two from 8 to 1024, not %d", k->page);
-    if (k->n_pages < 0 || k->kv_heads < 1 || k->kv_heads > 1024) return ops_say("cache: n_pages %d, kv_heads %d (1 .. 1024)", k->n_pages, k->kv_heads);
+    if (k->n_pages < 1 || k->kv_heads < 1 || k->kv_heads > 1024) return ops_say("cache: n_pages %d, kv_heads %d (1 .. 1024)", k->n_pages, k->kv_heads);
     if (k->page_stride < (int64_t)k->kv_heads * k->page * k->head_dim) return ops_say("page_stride %lld is shorter than a page", (long long)k->page_stride);
     if (k->page_stride > OPS_MAX_STRIDE) return "page_stride too large";
     if (odd16(k->k) || odd16(k->v) || odd16(k->page_stride, k->dtype)) return "cache pages must be 16-byte aligned";
@@ -86,7 +86,7 @@ static inline std::string check_attention(const hipvoc_kv_cache *cache, const vo
     const int64_t row = (int64_t)n_heads * cache->head_dim;
     if (q_stride < row || out_stride < row || q_stride > OPS_MAX_STRIDE || out_stride > OPS_MAX_STRIDE) return "q_stride / out_stride shorter than n_heads * head_dim";
     if (odd16(q) || odd16(out) || odd16(q_stride, dtype) || odd16(out_stride, dtype)) return "rows must be 16-byte aligned";
-    const AttnPlan p = attention_plan(cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
+    const AttnPlan p = attention_plan(dtype, cache->dtype != dtype, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
     if (p.bytes && (!workspace || odd16(workspace) || workspace_bytes < p.bytes))
         return ops_say("workspace: %zu bytes needed, 16-byte aligned (hipvoc_attention_workspace)", p.bytes);
     return "";

@@ -1,4 +1,4 @@
-// Index arithmetic of the token-step operators, the same on host and device: how a sequence is cut into chunks, which keys a chunk has, and
+// Index arithmetic of the token-step operators, the same on host and device: how a call's keys are cut, which of them a workgroup has, and
 // where a token's row is.  Pure C++, so that tests/native/fuzz_ops.cpp can check on the CPU that no length, offset or page number leads
 // out of bounds.
 #pragma once
@@ -13,21 +13,30 @@
 
 namespace hipvoc {
 
-// Keys [from, to) of chunk `c` of a sequence of n tokens, out of those its new token sees, [lo, hi); `active` chunks have any.  A length
-// outside 0 .. max_len is bad: no key is read, and chunk 0 is there to say so.
-struct AttnSpan { int lo, hi, from, to, active; bool bad; };
-OPS_FN AttnSpan attn_span(int n, int max_len, int window, int chunk, int c) {
+// ---- attention: which keys a token sees, and which of them a workgroup has ---------------------------------------------------------------
+// Keys come in tiles of 32, counted from `base`, the first seen key lo rounded down to a tile.  A length outside 0 .. max_len is bad: no
+// key is read.
+struct AttnSpan { int lo, hi, base, tiles; bool bad; };
+OPS_FN AttnSpan attn_span(int n, int max_len, int window) {
     AttnSpan s;
     s.bad = n < 0 || n > max_len;
     s.hi = s.bad ? 0 : n;
     s.lo = window > 0 && s.hi > window ? s.hi - window : 0;
-    const int base = s.lo & ~31;                            // chunks start on a multiple of the 32-key tile
-    s.active = s.bad ? 1 : (int)(((int64_t)s.hi - base + chunk - 1) / chunk);
-    const int64_t from = (int64_t)base + (int64_t)c * chunk, to = from + chunk;
-    s.from = (int)(from < s.hi ? from : s.hi);
-    s.to = (int)(to < s.hi ? to : s.hi);
+    s.base = s.lo & ~31;
+    s.tiles = (int)(((int64_t)s.hi - s.base + 31) / 32);
     return s;
 }
+
+// A call is cut over all its tiles at once: they stand in a row (sequence by sequence, in it head by head), `total` of them, and worker w of
+// `workers` (a wave, or a workgroup for 32-bit activations) has the tiles [first(w), first(w + 1)), whatever sequences they belong to.  So
+// sequences of unequal length load the card alike.  A piece (the part of one sequence and head that a worker has) leaves its state in slot
+// w + pair, pair = sequence * heads + head: along the row every piece has a larger w or a larger pair than the one before, so no two share one.
+OPS_FN int64_t attn_workers(int64_t total, int least, int most) {              // a worker has `least` tiles, if there are that many
+    const int64_t w = (total + least - 1) / least;
+    return w < most ? w : most;
+}
+OPS_FN int64_t attn_first(int64_t w, int64_t total, int64_t workers) { return w * total / workers; }
+OPS_FN int64_t attn_worker_of(int64_t tile, int64_t total, int64_t workers) { return ((tile + 1) * workers - 1) / total; }
 
 // Position of row t of a call in its sequence (rows start at cu, the first stands at position `first`); -1: not in the sequence's pages
 OPS_FN int64_t row_position(int t, int cu, int first, int table_width, int page_shift) {
@@ -36,21 +45,27 @@ OPS_FN int64_t row_position(int t, int cu, int first, int table_width, int page_
 }
 OPS_FN bool page_ok(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages; }
 
-struct AttnPlan { int chunk, n_chunks; size_t bytes; };
-// How a call is cut, from sizes alone.  The longest sequence decides the chunk; shorter ones have fewer of the same length.
-inline AttnPlan attention_plan(int head_dim, int kv_heads, int n_heads, int n_seqs, int max_len, int window) {
+struct AttnPlan { int heads, workers, least; size_t bytes; };
+enum { ATTN_MAX_SEQS = 1024, ATTN_WHOLE_TILES = 24 };      // sequences whose lengths a workgroup adds up; tiles that are not worth a cut
+// How a call is cut, from sizes alone.  `heads`: (key head, tile of query heads) pairs of a sequence; a workgroup each (workers 0) if the spans
+// are short, where joining would cost more than it gives, or the sequences so many that they fill the card.  Else the workers that the
+// card holds at a time share the tiles.
+inline AttnPlan attention_plan(int dtype, bool coded, int head_dim, int kv_heads, int n_heads, int n_seqs, int max_len, int window) {
     AttnPlan p;
-    const int64_t span = window > 0 && (int64_t)window + 31 < max_len ? (int64_t)window + 31 : max_len;
-    const int64_t pairs = (int64_t)n_seqs * kv_heads;
-    int64_t parts = 2048 / (pairs > 0 ? pairs : 1);
-    if (parts < 1) parts = 1;
-    int64_t chunk = (span + parts - 1) / parts;
-    chunk = (chunk + 127) / 128 * 128;
-    if (chunk < 256) chunk = 256;
-    p.chunk = (int)chunk;
-    p.n_chunks = (int)((span + chunk - 1) / chunk);
-    if (p.n_chunks < 1) p.n_chunks = 1;
-    p.bytes = p.n_chunks > 1 ? (size_t)n_seqs * n_heads * p.n_chunks * (head_dim + 2) * sizeof(float) : 0;
+    const bool f32 = dtype == 0;
+    const int group = n_heads / kv_heads, most = !f32 ? 16 : group < 3 ? group : 4;      // query heads of a pair
+    const int64_t span = window > 0 && (int64_t)window + 31 < max_len ? (int64_t)window + 31 : max_len, tiles = (span + 31) / 32;
+    p.heads = kv_heads * ((group + most - 1) / most);
+    p.least = f32 ? 8 : 1;
+    p.workers = 0;
+    p.bytes = 0;
+    if (tiles > ATTN_WHOLE_TILES && n_seqs <= ATTN_MAX_SEQS) {
+        const int64_t pairs = (int64_t)n_seqs * p.heads;
+        p.workers = (int)attn_workers(pairs * tiles, p.least, f32 ? 768 : coded ? 3072 : 2048);
+        // slots of up to `most` heads: (m, l) and the sums; then the row's length before each sequence
+        p.bytes = (size_t)(p.workers + pairs) * (size_t)(group < most ? group : most) * (size_t)(head_dim + 2) * sizeof(float);
+        p.bytes = (p.bytes + 15) / 16 * 16 + (size_t)(n_seqs + 1) * sizeof(int64_t);
+    }
     return p;
 }
 

@@ -40,9 +40,10 @@ struct AttnArgs {
     const int32_t *lens;
     int n_seqs, max_len, window;
     float scale_log2;                    // scale * log2(e): softmax in powers of two
-    // set by the launcher's plan
-    int chunk, n_chunks;                 // keys per workgroup, and the most parts a sequence has
-    float *part;                         // [n_seqs][n_heads][n_chunks][head_dim + 2] when n_chunks > 1
+    // the plan (ops_index.hpp)
+    int heads, workers, least;           // pairs per sequence; 0 workers: a workgroup per pair, nothing to join
+    float *part;                         // slots [workers + n_seqs * heads][query heads of a pair][head_dim], then (m, l) of each
+    int64_t *before;                     // [n_seqs + 1] tiles (of one pair) before each sequence
     int *err;
 };
 hipError_t launch_attention_decode(const AttnArgs &a, hipStream_t s);

@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <algorithm>
 #include <random>
 #include <string>
 #include <vector>
@@ -23,28 +24,56 @@ static int pick(int lo, int hi) { return std::uniform_int_distribution<int>(lo, 
 static void spans() {
     const int odd[] = {INT_MIN, -1, 0, 1, 31, 32, 33, 127, 128, 129, 255, 256, 257, 4095, 131071, INT_MAX - 256};
     for (int it = 0; it < 20000; it++) {
-        const int max_len = it % 3 ? pick(0, 200000) : odd[pick(2, 15)];
-        const int len = it % 5 == 0 ? odd[pick(0, 15)] : pick(0, max_len);
-        const int window = it % 2 ? 0 : it % 4 ? pick(1, 5000) : odd[pick(3, 15)];
-        const int heads = pick(1, 16), seqs = pick(1, 300);
-        const AttnPlan p = attention_plan(64, heads, heads * 2, seqs, max_len, window);
-        CHECK(p.chunk >= 256 && p.chunk % 128 == 0 && p.n_chunks >= 1);
-        CHECK((p.n_chunks > 1) == (p.bytes > 0));
-        int at = -1, found = 0;
-        const AttnSpan first = attn_span(len, max_len, window, p.chunk, 0);
-        CHECK(first.bad == (len < 0 || len > max_len));
-        CHECK(first.active <= p.n_chunks);                      // every chunk that has keys has a place in the workspace
-        for (int c = 0; c < p.n_chunks; c++) {
-            const AttnSpan s = attn_span(len, max_len, window, p.chunk, c);
-            CHECK(s.from <= s.to && s.to <= s.hi && s.hi <= (s.bad ? 0 : len) && s.lo >= 0 && s.lo <= s.hi);
-            if (s.bad) { CHECK(s.from == s.to); continue; }
-            if (c >= s.active) { CHECK(s.from == s.to); continue; }
-            CHECK(s.to > s.from && s.from % 32 == 0 && (at < 0 ? s.from <= s.lo && s.lo - s.from < 32 : s.from == at));
-            CHECK(s.to > s.lo);                                 // a key of the chunk is in sight, so that masked places can be read from it
-            at = s.to;
-            found += s.to - (s.from > s.lo ? s.from : s.lo);
+        const int max_len = it % 3 ? pick(0, 200000) : odd[pick(2, 15)], len = it % 2 ? odd[pick(0, 15)] : pick(0, max_len);
+        const int window = it % 5 ? 0 : odd[pick(3, 15)];
+        const AttnSpan s = attn_span(len, max_len, window);
+        CHECK(s.bad == (len < 0 || len > max_len));
+        if (s.bad) { CHECK(s.hi == 0 && s.lo == 0 && s.tiles == 0); continue; }
+        CHECK(s.hi == len && s.lo == (window > 0 && len > window ? len - window : 0));
+        CHECK(s.base % 32 == 0 && s.base <= s.lo && s.lo - s.base < 32 && s.tiles == (int)(((int64_t)len - s.base + 31) / 32));
+        CHECK((len == 0) == (s.tiles == 0));
+    }
+}
+
+// The row of tiles, as kernel and join walk it: every tile in one piece, every piece in a slot of its own inside the workspace, and a pair in one
+// piece exactly where the join thinks so.
+static void cuts() {
+    for (int it = 0; it < 3000; it++) {
+        const int seqs = it % 4 ? pick(1, 12) : pick(1, 300), kv = pick(1, 8), group = pick(1, 20), dtype = pick(0, 2), hd = it % 2 ? 64 : 128;
+        const int max_len = it % 7 ? pick(1, 40000) : pick(1, 400), window = it % 3 ? 0 : pick(1, 3000);
+        const AttnPlan p = attention_plan(dtype, it % 3 == 0, hd, kv, kv * group, seqs, max_len, window);
+        const int most = dtype ? 16 : group < 3 ? group : 4;
+        CHECK(p.heads == kv * ((group + most - 1) / most) && (p.bytes > 0) == (p.workers > 0));
+        if (!p.workers) continue;
+        std::vector<int64_t> before(seqs + 1, 0);
+        for (int b = 0; b < seqs; b++) before[b + 1] = before[b] + attn_span(pick(0, 9) ? pick(0, 5) ? pick(0, max_len) : pick(-3, 40) : max_len, max_len, window).tiles;
+        const int64_t total = before[seqs] * p.heads, workers = attn_workers(total, p.least, p.workers);
+        CHECK(workers <= p.workers && (workers > 0) == (total > 0));
+        if (!total) continue;
+        const int64_t slots = p.workers + (int64_t)seqs * p.heads, n = group < most ? group : most;
+        CHECK((size_t)(slots * n * (hd + 2)) * sizeof(float) + (seqs + 1) * sizeof(int64_t) <= p.bytes);
+        int64_t last_slot = -1, x = 0;
+        for (int64_t w = 0; w < workers; w++) {
+            CHECK(x == attn_first(w, total, workers));
+            const int64_t end = attn_first(w + 1, total, workers);
+            CHECK(end > x || total < workers);
+            while (x < end) {
+                int seq = 0;
+                for (int m = seqs; m > 1;) { const int half = m / 2; if (before[seq + half] * p.heads <= x) seq += half; m -= half; }
+                while (before[seq + 1] * p.heads <= x) seq++;
+                CHECK(seq < seqs && before[seq] * p.heads <= x);
+                const int64_t tiles = before[seq + 1] - before[seq], rest = x - before[seq] * p.heads, pair = rest / tiles, tile = rest % tiles;
+                CHECK(pair < p.heads);
+                const int64_t m = std::min(tiles - tile, end - x), slot = w + seq * (int64_t)p.heads + pair;
+                CHECK(slot > last_slot && slot < slots);
+                last_slot = slot;
+                const int64_t first = before[seq] * p.heads + pair * tiles, w0 = attn_worker_of(first, total, workers), w1 = attn_worker_of(first + tiles - 1, total, workers);
+                CHECK(w0 <= w && w <= w1 && (m == tiles) == (w0 == w1));
+                CHECK(attn_worker_of(x, total, workers) == w && attn_worker_of(x + m - 1, total, workers) == w);
+                x += m;
+            }
         }
-        if (!first.bad) CHECK(found == (window > 0 && len > window ? window : len));
+        CHECK(x == total);
     }
 }
 
@@ -209,6 +238,7 @@ static void products() {
 
 int main() {
     spans();
+    cuts();
     rows();
     caches();
     moves();

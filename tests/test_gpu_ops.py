@@ -395,7 +395,10 @@ def test_attention_deferred_errors(pkg, ops):
     out, lse = ops.attention(q, L.cache, L.table, ints([5001, 4000]), max_len=5000, lse=True)
     with pytest.raises(pkg.HipVocError):
         ops.sync()
-    assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all()) and torch.equal(out[1], good[1])
+    assert bool(out[0].isnan().all()) and bool(lse[0].isnan().all())
+    # the keys of a call are cut over all its sequences: without the first one's, the second's are added up in another order
+    ro, _, bo, _ = attention_ref(L, q.cpu(), 1 / 8, 0)
+    assert bool(((out[1].cpu().double() - ro[1]).abs() <= bo[1]).all())
     ops.sync()
 
 
