@@ -6,12 +6,16 @@
 // ones gives in the same registers.  No product has a rounding; all sums are in 32 bits.  32-bit rows are cut into three bf16 parts of 8
 // mantissa bits each (exactly x together), three matrix instructions for one.  8-bit rows: a code's two's complement of (c - 8) is moved to the
 // top of a byte, 16 (c - 8), the group's sum is an exact integer, and 1/16 is part of the scale.
-// Bound: memory, half a byte per weight read once; next to it the vector ALU, which turns 8 codes into operands with 8 instructions (4 for
-// 8-bit rows).
-// Layout: one wave has RT tiles of 16 weight rows, the workgroup's waves share the rows and take every NW-th slab of 128 columns: a lane
-// reads 16 bytes of one row.  x rows are the other side of the matrix instruction (up to 16 of them; rows behind the last repeat it and are
-// not stored), so a lane's four results belong to ONE weight row: one scale per lane and group.  With groups shorter than a slab the four lanes of
-// a row exchange their dwords (two permlane swaps) so that a matrix instruction's 32 columns are one group.
+// Bound: memory, half a byte per weight read once (non-temporal); next to it the vector ALU, which turns 8 codes into operands with 8 instructions
+// (5 for 8-bit rows), and the cache's line rate.  16 x 4096 x 65536 in f16 with groups of 64: 39 us, 4.0 TB/s; 1 x 1024 x 65536: 14 us.
+// Layout: one wave has RT tiles of 16 weight rows and slabs of 128 columns: a lane reads 16 bytes of one row, and the four lanes of a row exchange their
+// dwords (permlane swaps) so that a matrix instruction's 32 columns are one group.  x rows are the other side of the matrix instruction
+// (up to 16 of them; rows behind the last repeat it and are not stored), so a lane's four results belong to ONE weight row: one scale per
+// lane and group.  q4_kernel: the workgroup's waves share 16 RT rows and take every NW-th slab, x read by each for itself; q4_wide_kernel: for
+// many weight rows, x through LDS.
+#include <atomic>
+#include <type_traits>
+
 #include "ops_device.h"
 
 namespace hipvoc {
@@ -27,15 +31,20 @@ __device__ __forceinline__ void swap16(unsigned &a, unsigned &b) {      // odd r
     b = r[1];
 }
 
-// Eight codes of a dword as a matrix operand, in the order 0 4 1 5 2 6 3 7 (16-bit types) or 0 2 4 6 1 3 5 7 (bytes)
+// Eight codes of a dword as a matrix operand, in the order 0 4 1 5 2 6 3 7 (16-bit types; bytes: 0 2 4 6 1 3 5 7).  `e`: the bits of 16, twice, in a register (with two literals the mask and the or would be two instructions)
 template <int XT> struct Codes {
-    static __device__ __forceinline__ u32x4 of(unsigned w) {
+    static __device__ __forceinline__ unsigned sixteen() {
+        unsigned e = XT == HIPVOC_T_F16 ? 0x4c004c00u : 0x41804180u;
+        asm("" : "+v"(e));
+        return e;
+    }
+    static __device__ __forceinline__ u32x4 of(unsigned w, unsigned e) {
         if constexpr (XT == HIPVOC_T_F16) {
-            constexpr unsigned M = 0x03c003c0u, E = 0x4c004c00u;
-            return (u32x4){((w << 6) & M) | E, ((w << 2) & M) | E, ((w >> 2) & M) | E, ((w >> 6) & M) | E};
+            constexpr unsigned M = 0x03c003c0u;
+            return (u32x4){((w << 6) & M) | e, ((w << 2) & M) | e, ((w >> 2) & M) | e, ((w >> 6) & M) | e};
         } else {
-            constexpr unsigned M = 0x00780078u, E = 0x41804180u;
-            return (u32x4){((w << 3) & M) | E, ((w >> 1) & M) | E, ((w >> 5) & M) | E, ((w >> 9) & M) | E};
+            constexpr unsigned M = 0x00780078u;
+            return (u32x4){((w << 3) & M) | e, ((w >> 1) & M) | e, ((w >> 5) & M) | e, ((w >> 9) & M) | e};
         }
     }
 };
@@ -52,16 +61,18 @@ __device__ __forceinline__ f32x4 mfma16(bool f16, u32x4 a, u32x4 b, f32x4 c) {
 template <int XT> struct XRow {
     static constexpr int P = XT == HIPVOC_T_F32 ? 3 : 1;
     u32x4 raw[XT == HIPVOC_T_F32 ? 2 : 1];
-    __device__ __forceinline__ void load(const void *x, int64_t at) {
-        if constexpr (XT == HIPVOC_T_F32) {
-            raw[0] = *(const u32x4 *)((const float *)x + at);
-            raw[1] = *(const u32x4 *)((const float *)x + at + 4);
-        } else if constexpr (XT == HIPVOC_T_INT8) {
-            const u32x2 v = *(const u32x2 *)((const uint8_t *)x + at);
+    __device__ __forceinline__ void load(const void *x) {
+        if constexpr (XT == HIPVOC_T_INT8) {
+            const u32x2 v = *(const u32x2 *)x;
             raw[0] = (u32x4){v[0], v[1], 0u, 0u};
         } else {
-            raw[0] = *(const u32x4 *)((const uint16_t *)x + at);
+            raw[0] = ((const u32x4 *)x)[0];
+            if constexpr (XT == HIPVOC_T_F32) raw[1] = ((const u32x4 *)x)[1];
         }
+    }
+    __device__ __forceinline__ void parts(long *p) const {
+        const u32x2 r = {__builtin_amdgcn_perm(raw[0][1], raw[0][0], 0x06040200), __builtin_amdgcn_perm(raw[0][1], raw[0][0], 0x07050301)};
+        p[0] = __builtin_bit_cast(long, r);
     }
     __device__ __forceinline__ void parts(u32x4 *p) const {
         if constexpr (XT == HIPVOC_T_F32) {
@@ -85,158 +96,156 @@ template <int XT> struct XRow {
             p[0] = order16(raw[0]);
         }
     }
-    __device__ __forceinline__ long bytes() const {
-        const u32x2 r = {__builtin_amdgcn_perm(raw[0][1], raw[0][0], 0x06040200), __builtin_amdgcn_perm(raw[0][1], raw[0][0], 0x07050301)};
-        return __builtin_bit_cast(long, r);
-    }
 };
 
-static constexpr int Q4_WAVES = 8;
+#ifndef Q4_RTB
+#define Q4_RTB 2
+#define Q4_KWB 2
+#endif
+#ifndef Q4_WIDE
+#define Q4_WIDE 16384
+#endif
+static constexpr int Q4_WAVES = 8, Q4_HALVES = 2, Q4_GROUPS = 128;      // waves of a workgroup; of the wide kernel, on how many shares of a block's slabs; groups of a row whose scales are in LDS at a time
 
 // What a wave reads of one slab of 128 columns
-template <int XT, int G, bool MINS, int RT> struct Slab {
-    static constexpr int NG = 128 / G;
+template <int XT, int RT> struct Slab {
     u32x4 w[RT];
     XRow<XT> x[4];
-    float s[RT][NG], least[RT][MINS ? NG : 1], sx[XT == HIPVOC_T_INT8 ? 4 : 1][NG];
 };
 
-template <int XT, int G, bool MINS, int RT>
-__device__ __forceinline__ void q4_load(const Q4Args &a, Slab<XT, G, MINS, RT> &b, int k0, int n0, int m0, int lane) {
-    constexpr int NG = 128 / G;
-    const int r16 = lane & 15, j = lane >> 4, groups = a.n_in / G, g0 = k0 / G;
-    const bool whole = k0 + 128 <= a.n_in;
-    const int xm = min(m0 + r16, a.n_rows - 1);
+// Where a lane reads: its rows of the weights and of x.  Slab s is 64 bytes of codes and 128 values on.
+template <int XT, int RT> struct Rows {
+    const uint8_t *w[RT];
+    const char *x;
+};
+template <int XT> constexpr int x_bytes() { return XT == HIPVOC_T_F32 ? 4 : XT == HIPVOC_T_INT8 ? 1 : 2; }
+
+template <int XT, int RT>
+__device__ __forceinline__ void q4_load(const Q4Args &a, const Rows<XT, RT> &r, Slab<XT, RT> &b, int s, int lane) {
+    const int j = lane >> 4;
+    constexpr int XB = x_bytes<XT>();
+    const char *x = r.x + ((int64_t)s * 128 + 8 * j) * XB;
+    if (s * 128 + 128 <= a.n_in) {
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int n = min(n0 + 16 * t + r16, a.n_out - 1);
-        const int64_t row = (int64_t)n * (a.n_in / 2);
-        const int at = k0 + 32 * j < a.n_in ? k0 / 2 + 16 * j : k0 / 2;           // a column behind the last belongs to no group that is used
-        b.w[t] = *(const u32x4 *)(a.codes + row + at);
-        const int64_t sc = (int64_t)n * groups + g0;
+        for (int t = 0; t < RT; t++) b.w[t] = __builtin_nontemporal_load((const u32x4 *)(r.w[t] + (int64_t)s * 64 + 16 * j));
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const int64_t i = sc + (whole || g0 + g < groups ? g : 0);
-            b.s[t][g] = (float)((const _Float16 *)a.scales)[i];
-            if constexpr (MINS) b.least[t][g] = (float)((const _Float16 *)a.mins)[i];
-        }
-    }
+        for (int c = 0; c < 4; c++) b.x[c].load(x + c * 32 * XB);
+    } else {                                                                      // a group behind the last is not used: read the slab's first instead
+        const int have = (a.n_in - s * 128) / 32;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int k = G == 128 ? k0 + 32 * j + 8 * c : k0 + (whole || k0 + 32 * c < a.n_in ? 32 * c : 0) + 8 * j;
-        b.x[c].load(a.x, xm * a.x_stride + k);
-    }
-    if constexpr (XT == HIPVOC_T_INT8) {
-        if (a.x_groups > 1) {
+        for (int t = 0; t < RT; t++) b.w[t] = __builtin_nontemporal_load((const u32x4 *)(r.w[t] + (int64_t)s * 64 + (j < have ? 16 * j : 0)));
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int64_t row = (int64_t)min(m0 + 4 * j + r, a.n_rows - 1) * groups + g0;
-#pragma unroll
-                for (int g = 0; g < NG; g++) b.sx[r][g] = a.x_scale[row + (whole || g0 + g < groups ? g : 0)];
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int g = 0; g < NG; g++) b.sx[r][g] = 1.f;                    // one scale per row: at the end
-        }
+        for (int c = 0; c < 4; c++) b.x[c].load(x + (c < have ? c : 0) * 32 * XB);
     }
 }
 
-template <int XT, int G, bool MINS, int RT>
-__device__ __forceinline__ void q4_use(const Q4Args &a, Slab<XT, G, MINS, RT> &b, int k0, f32x4 (&out)[RT]) {
+// sc: (scale, least value), two f16, of the slab's first group for this lane's row of tile 0; tile t is t * 16 rows of `stride` further on.
+// sx: the scales of x rows 4j .. 4j + 3 for the slab's first group
+// x(c, part) is the operand of 32 columns c.
+template <int XT, int G, bool MINS, int RT, typename X>
+__device__ __forceinline__ void q4_use(const Q4Args &a, u32x4 (&w)[RT], X &&x, int k0, const h16x2 *sc, int stride, const f32x4 *sx, f32x4 (&out)[RT]) {
     constexpr int NG = 128 / G, PER = 4 / NG;                                     // matrix instructions of 32 columns per group
-    const bool whole = k0 + 128 <= a.n_in;
-    if constexpr (G < 128) {
+    {
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            unsigned d[4] = {b.w[t][0], b.w[t][1], b.w[t][2], b.w[t][3]};
+            unsigned d[4] = {w[t][0], w[t][1], w[t][2], w[t][3]};
             swap32(d[0], d[2]);
             swap32(d[1], d[3]);
             swap16(d[0], d[1]);
             swap16(d[2], d[3]);
-            b.w[t] = (u32x4){d[0], d[1], d[2], d[3]};
+            w[t] = (u32x4){d[0], d[1], d[2], d[3]};
         }
     }
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        if (!whole && k0 + g * G >= a.n_in) break;
+    const auto group = [&](int g) {
         if constexpr (XT == HIPVOC_T_INT8) {
             i32x4 acc[RT] = {}, sum = {};
 #pragma unroll
             for (int p = 0; p < PER; p++) {
                 const int c = g * PER + p;
-                const long x = b.x[c].bytes();
-                if constexpr (MINS) sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(x, 0x0101010101010101L, sum, 0, 0, 0);
+                long xc[1];
+                x(c, xc);
+                if constexpr (MINS) sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(xc[0], 0x0101010101010101L, sum, 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const unsigned w = b.w[t][c] ^ 0x88888888u;
-                    const u32x2 v = {(w << 4) & 0xf0f0f0f0u, w & 0xf0f0f0f0u};
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x, __builtin_bit_cast(long, v), acc[t], 0, 0, 0);
+                    const unsigned v = w[t][c] ^ 0x88888888u;
+                    const u32x2 wc = {(v << 4) & 0xf0f0f0f0u, v & 0xf0f0f0f0u};
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xc[0], __builtin_bit_cast(long, wc), acc[t], 0, 0, 0);
                 }
             }
+            f32x4 xs = {1.f, 1.f, 1.f, 1.f};
+            if (a.x_groups > 1) xs = sx[4 * g];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-                const float s = b.s[t][g] * 0.0625f;
+                const h16x2 p = sc[t * 16 * stride + g];
+                const float s = (float)p[0] * 0.0625f, off = MINS ? fmaf(128.f, s, (float)p[1]) : 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     float v = s * (float)acc[t][r];
-                    if constexpr (MINS) v = fmaf(fmaf(8.f, b.s[t][g], b.least[t][g]), (float)sum[r], v);
-                    out[t][r] = fmaf(b.sx[r][g], v, out[t][r]);
+                    if constexpr (MINS) v = fmaf(off, (float)sum[r], v);
+                    out[t][r] = fmaf(xs[r], v, out[t][r]);
                 }
             }
         } else {
             constexpr bool F16 = XT == HIPVOC_T_F16;
             constexpr unsigned ONE = F16 ? 0x3c003c00u : 0x3f803f80u;
             const u32x4 ones = {ONE, ONE, ONE, ONE};
+            const unsigned e16 = Codes<XT>::sixteen();
             f32x4 acc[RT] = {}, sum = {};
 #pragma unroll
             for (int p = 0; p < PER; p++) {
                 const int c = g * PER + p;
-                u32x4 x[XRow<XT>::P];
-                b.x[c].parts(x);
+                u32x4 xc[XRow<XT>::P];
+                x(c, xc);
 #pragma unroll
-                for (int i = 0; i < XRow<XT>::P; i++) sum = mfma16(F16, x[i], ones, sum);
+                for (int i = 0; i < XRow<XT>::P; i++) sum = mfma16(F16, xc[i], ones, sum);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const u32x4 w = Codes<XT>::of(b.w[t][c]);
+                    const u32x4 wc = Codes<XT>::of(w[t][c], e16);
 #pragma unroll
-                    for (int i = 0; i < XRow<XT>::P; i++) acc[t] = mfma16(F16, x[i], w, acc[t]);
+                    for (int i = 0; i < XRow<XT>::P; i++) acc[t] = mfma16(F16, xc[i], wc, acc[t]);
                 }
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-                const float s = b.s[t][g], off = MINS ? fmaf(-16.f, s, b.least[t][g]) : -24.f * s;
+                const h16x2 p = sc[t * 16 * stride + g];
+                const float s = (float)p[0], off = MINS ? fmaf(-16.f, s, (float)p[1]) : -24.f * s;
 #pragma unroll
                 for (int r = 0; r < 4; r++) out[t][r] = fmaf(s, acc[t][r], fmaf(off, sum[r], out[t][r]));
             }
         }
+    };
+    if (k0 + 128 <= a.n_in) {                                                     // no branch between the groups of a whole slab
+#pragma unroll
+        for (int g = 0; g < NG; g++) group(g);
+    } else {
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+            if (k0 + g * G < a.n_in) group(g);
     }
 }
 
-template <int XT, int G, bool MINS, int RT>
-__global__ __launch_bounds__(64 * Q4_WAVES) void q4_kernel(Q4Args a) {
-    __shared__ float red[Q4_WAVES][16][16 * RT + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 16, slabs = (a.n_in + 127) / 128;
-    f32x4 out[RT] = {};
-    Slab<XT, G, MINS, RT> cur, next;
-    if (wave < slabs) q4_load(a, cur, wave * 128, n0, m0, lane);
-    for (int s = wave; s < slabs; s += nw) {
-        if (s + nw < slabs) q4_load(a, next, (s + nw) * 128, n0, m0, lane);
-        q4_use(a, cur, s * 128, out);
-        cur = next;
-    }
+__host__ __device__ constexpr int q4_stride(int held) { return held + 1 + (held & 1); }      // odd: 16 rows in 16 banks
+static size_t q4_lds(bool int8, int rows, int groups, int kw) {
+    const int held = groups < Q4_GROUPS ? groups : Q4_GROUPS;
+    const size_t scales = (int8 ? (size_t)held * 64 : 0) + (size_t)rows * q4_stride(held) * 4, sums = (size_t)kw * 16 * (rows + 1) * 4;
+    return scales > sums ? scales : sums;
+}
+
+// Adds the waves' sums up and stores them
+template <int XT, int RT>
+__device__ __forceinline__ void q4_finish(const Q4Args &a, const f32x4 (&out)[RT], float *red, int kw, int part, int row0, int wg_rows, int n0, int m0) {
+    const int lane = threadIdx.x & 63, r16 = lane & 15, j = lane >> 4;
+    __syncthreads();                                                              // the scales' place is free
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) red[wave][4 * (lane >> 4) + r][16 * t + (lane & 15)] = out[t][r];
+        for (int r = 0; r < 4; r++) red[(part * 16 + 4 * j + r) * (wg_rows + 1) + row0 + 16 * t + r16] = out[t][r];
     __syncthreads();
-    for (int i = threadIdx.x; i < 256 * RT; i += blockDim.x) {
-        const int n = n0 + i % (16 * RT), ml = i / (16 * RT), m = m0 + ml;
+    for (int i = threadIdx.x; i < 16 * wg_rows; i += blockDim.x) {
+        const int ml = i / wg_rows, nl = i - ml * wg_rows, n = n0 + nl, m = m0 + ml;
         if (n >= a.n_out || m >= a.n_rows) continue;
         float v = 0.f;
-        for (int w = 0; w < nw; w++) v += red[w][ml][i % (16 * RT)];
+        for (int w = 0; w < kw; w++) v += red[(w * 16 + ml) * (wg_rows + 1) + nl];
         if constexpr (XT == HIPVOC_T_INT8) {
             if (a.x_groups == 1) v *= a.x_scale[m];
         }
@@ -247,20 +256,213 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void q4_kernel(Q4Args a) {
     }
 }
 
-template <int XT, int G, bool MINS> static void q4_rt(const Q4Args &a, hipStream_t s) {
-    const int slabs = (a.n_in + 127) / 128, nw = slabs < Q4_WAVES ? slabs : Q4_WAVES, tiles = (a.n_out + 15) / 16, my = (a.n_rows + 15) / 16;
-    if (tiles >= 1024) q4_kernel<XT, G, MINS, 2><<<dim3((tiles + 1) / 2, my), 64 * nw, 0, s>>>(a);
-    else q4_kernel<XT, G, MINS, 1><<<dim3(tiles, my), 64 * nw, 0, s>>>(a);
+// The scales of the workgroup's rows (and of x's, for 8-bit rows) of up to Q4_GROUPS groups, into LDS: read once in whole lines by all waves (a lane's
+// own reads would touch 16 lines for 32 bytes, in every slab)
+template <int XT, bool MINS>
+__device__ __forceinline__ void q4_stage_scales(const Q4Args &a, h16x2 *scales, float (*x_scales)[16], int n0, int m0, int wg_rows, int groups, int g0, int stride) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, n = min(Q4_GROUPS, groups - g0);
+            if (groups % 8 == 0 && groups <= Q4_GROUPS) {                                 // the rows are one piece of memory: eight groups a load
+        const int per_row = groups / 8, count = min(wg_rows, a.n_out - n0) * per_row, step = blockDim.x;
+        const u32x4 *s = (const u32x4 *)((const _Float16 *)a.scales + (int64_t)n0 * groups), *l = (const u32x4 *)((const _Float16 *)a.mins + (int64_t)n0 * groups);
+        for (int first = threadIdx.x; first < count; first += 4 * step) {
+            u32x4 v[4], m[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = min(first + i * step, count - 1);
+                v[i] = s[at];
+                m[i] = MINS ? l[at] : (u32x4){0u, 0u, 0u, 0u};
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = first + i * step, row = at / per_row, g = (at - row * per_row) * 8;
+                if (at < count) {
+                    unsigned *to = (unsigned *)scales + row * stride + g;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) to[e] = __builtin_amdgcn_perm(m[i][e >> 1], v[i][e >> 1], e & 1 ? 0x07060302 : 0x05040100);
+                }
+            }
+        }
+    } else
+    for (int first = wave; first < wg_rows; first += 8 * nw) {               // eight rows' loads at a time: one latency
+                _Float16 v[8][2], m[8][2];
+    #pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int64_t at = (int64_t)min(n0 + first + i * nw, a.n_out - 1) * groups + g0;
+    #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int g = min(lane + 64 * h, n - 1);
+                        v[i][h] = ((const _Float16 *)a.scales)[at + g];
+                        m[i][h] = MINS ? ((const _Float16 *)a.mins)[at + g] : (_Float16)0.f;
+                    }
+                }
+    #pragma unroll
+                for (int i = 0; i < 8; i++)
+    #pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (first + i * nw < wg_rows && lane + 64 * h < n) scales[(first + i * nw) * stride + lane + 64 * h] = (h16x2){v[i][h], m[i][h]};
+            }
+    if constexpr (XT == HIPVOC_T_INT8) {
+        if (a.x_groups > 1)
+            for (int row = wave; row < 16; row += nw) {
+                const int64_t at = (int64_t)min(m0 + row, a.n_rows - 1) * groups + g0;
+                for (int g = lane; g < n; g += 64) x_scales[g][row] = a.x_scale[at + g];
+            }
+    }
 }
-template <int XT, int G> static void q4_mins(const Q4Args &a, hipStream_t s) {
-    if (a.mins) q4_rt<XT, G, true>(a, s);
-    else q4_rt<XT, G, false>(a, s);
+
+template <int XT, int G, bool MINS, int RT>
+__global__ __launch_bounds__(64 * Q4_WAVES) void q4_kernel(Q4Args a, int kw) {
+    constexpr bool INT8 = XT == HIPVOC_T_INT8;
+    // LDS: the scales of x (8-bit rows), those of the weights, and at the end, in their place, the waves' sums (q4_lds)
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, r16 = lane & 15, j = lane >> 4;
+    const int part = wave % kw, row0 = wave / kw * 16 * RT, wg_rows = nw / kw * 16 * RT;
+    const int n0 = blockIdx.x * wg_rows, m0 = blockIdx.y * 16, slabs = (a.n_in + 127) / 128, groups = a.n_in / G;
+    const int held = min(groups, Q4_GROUPS), stride = q4_stride(held);
+    float (*x_scales)[16] = (float (*)[16])lds;
+    h16x2 *scales = (h16x2 *)(lds + (INT8 ? held * 64 : 0));
+    float *red = (float *)lds;                                                    // [kw][16][wg_rows + 1]
+    f32x4 out[RT] = {};
+    Slab<XT, RT> cur, next;
+    Rows<XT, RT> rows;
+#pragma unroll
+    for (int t = 0; t < RT; t++) rows.w[t] = a.codes + (int64_t)min(n0 + row0 + 16 * t + r16, a.n_out - 1) * (a.n_in / 2);
+    rows.x = (const char *)a.x + min(m0 + r16, a.n_rows - 1) * a.x_stride * x_bytes<XT>();
+    if (part < slabs) q4_load<XT, RT>(a, rows, cur, part, lane);
+    for (int g0 = 0; g0 < groups; g0 += Q4_GROUPS) {
+        if (g0) __syncthreads();
+        q4_stage_scales<XT, MINS>(a, scales, x_scales, n0, m0, wg_rows, groups, g0, stride);
+        __syncthreads();
+        const int last = min(slabs, (g0 + Q4_GROUPS) * G / 128);
+        for (int i = g0 * G / 128 + part; i < last; i += kw) {
+            if (i + kw < slabs) q4_load<XT, RT>(a, rows, next, i + kw, lane);
+            const int g = i * 128 / G - g0;
+            q4_use<XT, G, MINS, RT>(a, cur.w, [&](int c, auto *o) { cur.x[c].parts(o); }, i * 128, &scales[(row0 + r16) * stride + g], stride, INT8 ? (const f32x4 *)&x_scales[g][4 * j] : nullptr, out);
+            cur = next;
+        }
+    }
+    q4_finish<XT, RT>(a, out, red, kw, part, row0, wg_rows, n0, m0);
 }
-template <int XT> static hipError_t q4_group(const Q4Args &a, hipStream_t s) {
-    if (a.group == 32) q4_mins<XT, 32>(a, s);
-    else if (a.group == 64) q4_mins<XT, 64>(a, s);
-    else q4_mins<XT, 128>(a, s);
+
+// Many rows of weights: x goes through LDS.  A matrix operand's 16 rows of x are 16 lines for one load of 1 KB, and the cache serves a line in about
+// four cycles whatever is taken of it: read by every wave for itself, x cost more than the weights (79 / 54 / 47 us for 1 / 2 / 4 tiles per
+// read of x; 65536 x 4096, 16 rows).  Here all waves read it along its rows, a block of BS slabs ahead, and lay it down in operand order.
+template <int XT, int G, bool MINS, int RT>
+__global__ __launch_bounds__(64 * Q4_WAVES) void q4_wide_kernel(Q4Args a) {
+    constexpr int kw = Q4_HALVES;
+    constexpr bool INT8 = XT == HIPVOC_T_INT8;
+    constexpr int BS = XT == HIPVOC_T_F32 ? 2 : 8, MINE = BS / kw, P = XRow<XT>::P, UNITS = BS * 256 / (64 * Q4_WAVES);     // slabs of a block, of them a wave's own; what a thread lays down of x
+    typedef typename std::conditional<INT8, long, u32x4>::type op_t;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = Q4_WAVES, r16 = lane & 15, j = lane >> 4;
+    const int part = wave % kw, row0 = wave / kw * 16 * RT, wg_rows = nw / kw * 16 * RT;
+    const int n0 = blockIdx.x * wg_rows, m0 = blockIdx.y * 16, slabs = (a.n_in + 127) / 128, groups = a.n_in / G;
+    const int held = min(groups, Q4_GROUPS), stride = q4_stride(held);
+    op_t *xl = (op_t *)lds;                                                       // [BS slabs][4][P][64 lanes]
+    float (*x_scales)[16] = (float (*)[16])(lds + BS * 256 * P * sizeof(op_t));
+    h16x2 *scales = (h16x2 *)(lds + BS * 256 * P * sizeof(op_t) + (INT8 ? held * 64 : 0));
+    float *red = (float *)lds;
+    XRow<XT> ahead[UNITS];
+    const auto fetch = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            const int u = tid + i * 64 * Q4_WAVES, m = u / (BS * 16), k = s0 * 128 + u % (BS * 16) * 8;
+            ahead[i].load((const char *)a.x + (min(m0 + m, a.n_rows - 1) * a.x_stride + (k < a.n_in ? k : 0)) * x_bytes<XT>());
+        }
+    };
+    // row m of eight columns q stands at m ^ q % 16: sixteen threads that write one row's columns, and sixteen that read one column's rows, hit all
+    // banks once
+    const auto lay = [&]() {
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            const int u = tid + i * 64 * Q4_WAVES, m = u / (BS * 16), q = u % (BS * 16);       // q: eight columns; 16 of them a slab, 4 an operand
+            op_t o[P];
+            ahead[i].parts(o);
+#pragma unroll
+            for (int p = 0; p < P; p++) xl[((q >> 2) * P + p) * 64 + (q & 3) * 16 + (m ^ (q & 15))] = o[p];
+        }
+    };
+    f32x4 out[RT] = {};
+    u32x4 w[MINE][RT];                                                            // a block's codes, each asked for again for the next block once used
+    const uint8_t *rows[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) rows[t] = a.codes + (int64_t)min(n0 + row0 + 16 * t + r16, a.n_out - 1) * (a.n_in / 2);
+    const auto load = [&](u32x4 (&w)[RT], int s) {
+        const int at = s * 64 + (s * 128 + 32 * j < a.n_in ? 16 * j : 0);
+#pragma unroll
+        for (int t = 0; t < RT; t++) w[t] = __builtin_nontemporal_load((const u32x4 *)(rows[t] + at));
+    };
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < MINE; i++)
+        if (part + i * kw < slabs) load(w[i], part + i * kw);
+    for (int s0 = 0; s0 < slabs; s0 += BS) {
+        const int g0 = s0 * 128 / G;
+        if (s0) __syncthreads();                                                  // the last block is used up
+        lay();
+        if (g0 % Q4_GROUPS == 0) q4_stage_scales<XT, MINS>(a, scales, x_scales, n0, m0, wg_rows, groups, g0, stride);
+        __syncthreads();
+        if (s0 + BS < slabs) fetch(s0 + BS);
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            const int s = s0 + part + i * kw;
+            if (s >= slabs) break;
+            const int g = (s * 128 / G) % Q4_GROUPS;
+            const op_t *xs = xl + (s - s0) * 4 * P * 64 + 16 * j;
+            q4_use<XT, G, MINS, RT>(a, w[i], [&](int c, op_t *o) {
+#pragma unroll
+                for (int p = 0; p < P; p++) o[p] = xs[(c * P + p) * 64 + (r16 ^ (4 * c + j))];
+            }, s * 128, &scales[(row0 + r16) * stride + g], stride, INT8 ? (const f32x4 *)&x_scales[g][4 * j] : nullptr, out);
+            if (s + BS < slabs) load(w[i], s + BS);
+        }
+    }
+    q4_finish<XT, RT>(a, out, red, kw, part, row0, wg_rows, n0, m0);
+}
+
+template <int XT, int G, bool MINS, int RT> static hipError_t q4_wide(const Q4Args &a, hipStream_t s) {
+    constexpr int rows = 16 * RT * Q4_WAVES / Q4_HALVES;
+    const size_t x = XT == HIPVOC_T_F32 ? 24576 : XT == HIPVOC_T_INT8 ? 16384 : 32768, lds = x + q4_lds(XT == HIPVOC_T_INT8, rows, a.n_in / G, Q4_HALVES);
+    const auto kernel = q4_wide_kernel<XT, G, MINS, RT>;
+    if (lds > 65536) {                                                            // over the default of a launch: said once per device
+        static std::atomic<bool> said[64];
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e == hipSuccess && (dev >= 64 || !said[dev].load())) {
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            if (e == hipSuccess && dev < 64) said[dev] = true;
+        }
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<dim3((a.n_out + rows - 1) / rows, (a.n_rows + 15) / 16), 64 * Q4_WAVES, lds, s>>>(a);
     return hipGetLastError();
+}
+// Which kernel, by the number of weight rows (4096 columns, groups of 64, 1 / 16 rows of x; us).  A workgroup of the wide kernel is slow by itself (it
+// takes 64 RT rows through four blocks), so it needs enough rows to fill 256 CUs:
+//    8192 rows: direct 8.7 / 13    wide<1> 15 / 15        16384: direct 16 / 23    wide<1> 16 / 16
+//   32768:      direct 29 / 43     wide<1> 22 / 23   wide<2> 22 / 23   wide<4> 33 / 34
+//   65536:      direct 56 / 84     wide<1> 41 / 44   wide<2> 43 / 45   wide<4> 37 / 39
+// 32-bit rows (three matrix instructions for one, blocks of two slabs), 4 rows of x: 16384: direct<1> 35, direct<2> 22, wide<2> 37; 65536: direct<2> 83,
+// wide<2> 56, wide<4> 54.
+template <int XT, int G, bool MINS> static hipError_t q4_rt(const Q4Args &a, hipStream_t s) {
+    const int slabs = (a.n_in + 127) / 128, kw = slabs < Q4_WAVES ? slabs : Q4_WAVES;
+    const auto direct = [&](int rt, auto kernel) {
+        kernel<<<dim3((a.n_out + 16 * rt - 1) / (16 * rt), (a.n_rows + 15) / 16), 64 * kw, q4_lds(XT == HIPVOC_T_INT8, 16 * rt, a.n_in / G, kw), s>>>(a, kw);
+        return hipGetLastError();
+    };
+    if constexpr (XT == HIPVOC_T_F32) {
+        if (a.n_out >= 32768) return q4_wide<XT, G, MINS, 2>(a, s);
+        if (a.n_out >= 8192) return direct(2, q4_kernel<XT, G, MINS, 2>);
+    } else {
+        if (a.n_out >= 65536) return q4_wide<XT, G, MINS, 4>(a, s);
+        if (a.n_out >= 16384) return q4_wide<XT, G, MINS, 1>(a, s);
+    }
+    return direct(1, q4_kernel<XT, G, MINS, 1>);
+}
+template <int XT, int G> static hipError_t q4_mins(const Q4Args &a, hipStream_t s) { return a.mins ? q4_rt<XT, G, true>(a, s) : q4_rt<XT, G, false>(a, s); }
+template <int XT> static hipError_t q4_group(const Q4Args &a, hipStream_t s) {
+    if (a.group == 32) return q4_mins<XT, 32>(a, s);
+    if (a.group == 64) return q4_mins<XT, 64>(a, s);
+    return q4_mins<XT, 128>(a, s);
 }
 hipError_t launch_q4_matvec(const Q4Args &a, hipStream_t s) {
     if (a.x_dtype == HIPVOC_T_INT8) return q4_group<HIPVOC_T_INT8>(a, s);
