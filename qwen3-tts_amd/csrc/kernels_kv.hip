@@ -41,83 +41,105 @@ __device__ __forceinline__ KvSlot kv_slot(const KvMoveArgs &a, int t, int lane, 
     return s;
 }
 
+// A wave takes KV_U times 64 lanes' worth of its token's rows, all their loads ahead of the question where they belong
+static constexpr int KV_U = 4;
+
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvMoveArgs a, int chunks) {
+__global__ __launch_bounds__(256) void kv_write_kernel(KvMoveArgs a, int parts) {
     constexpr int LPR = HD / 8, RPW = 64 / LPR;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, t = (int)(w / chunks), row = (int)(w % chunks) * RPW + lane / LPR, d = (lane % LPR) * 8;
+    const int lane = threadIdx.x & 63, t = (int)(w / parts), row0 = (int)(w % parts) * RPW * KV_U + lane / LPR, d = (lane % LPR) * 8;
     if (t >= a.n_rows) return;
-    const bool mine = row < 2 * a.c.kv_heads, value = row >= a.c.kv_heads;
-    const int head = value ? row - a.c.kv_heads : row;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    Raw8<ACT> raw;
     typedef typename Store<ACT>::type act_t;
-    if (mine) {
-        const act_t *src = (const act_t *)(value ? a.v : a.k) + t * (value ? a.v_stride : a.k_stride) + head * HD + d;
-        if constexpr (ST == ACT) raw = load_raw8<ACT>(src);
-        else load8<ACT>(src, x);
+    typedef typename Store<ST>::type st_t;
+    Raw8<ACT> raw[KV_U];
+#pragma unroll
+    for (int u = 0; u < KV_U; u++) {
+        const int row = row0 + u * RPW, value = row >= a.c.kv_heads, head = value ? row - a.c.kv_heads : row;
+        if (row < 2 * a.c.kv_heads) raw[u] = load_raw8<ACT>((const act_t *)(value ? a.v : a.k) + t * (value ? a.v_stride : a.k_stride) + head * HD + d);
     }
     bool padding;
     const KvSlot s = kv_slot(a, t, lane, padding);
     if (!s.in) return;                                                   // the whole wave: a wave has one token
-    typedef typename Store<ST>::type st_t;
-    st_t *dst = (st_t *)(value ? a.c.v : a.c.k) + s.row + (int64_t)head * a.c.page * HD + d;
-    if constexpr (ST == ACT) {
-        if (mine) store_raw8<ACT>(dst, raw);
-    } else {
-        float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = amax_nan(m, x[i]);
+    for (int u = 0; u < KV_U; u++) {
+        const int row = row0 + u * RPW, value = row >= a.c.kv_heads, head = value ? row - a.c.kv_heads : row;
+        const bool mine = row < 2 * a.c.kv_heads;
+        st_t *dst = (st_t *)(value ? a.c.v : a.c.k) + s.row + (int64_t)head * a.c.page * HD + d;
+        if constexpr (ST == ACT) {
+            if (mine) store_raw8<ACT>(dst, raw[u]);
+        } else {
+            float x[8];
+            load8<ACT>(&raw[u], x);
+            unsigned m = 0;
 #pragma unroll
-        for (int o = 1; o < LPR; o *= 2) m = amax_nan(m, __shfl_xor(m, o));
-        const float scale = scale8<ST>(m);
-        if (mine) {
-            *(u32x2 *)dst = codes8<ST>(x, scale);
-            if (d == 0) (value ? a.c.v_scale : a.c.k_scale)[s.scale + (int64_t)head * a.c.page] = scale;
+            for (int i = 0; i < 8; i++) m = amax_bits(m, x[i]);
+            const float scale = scale8<ST>(__uint_as_float(amax_lanes(m, LPR)));
+            if (mine) {
+                *(u32x2 *)dst = Coder<ST>(scale).eight(x);
+                if (d == 0) (value ? a.c.v_scale : a.c.k_scale)[s.scale + (int64_t)head * a.c.page] = scale;
+            }
         }
     }
 }
 
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvMoveArgs a, int chunks) {
+__global__ __launch_bounds__(256) void kv_read_kernel(KvMoveArgs a, int parts) {
     constexpr int LPR = HD / 8, RPW = 64 / LPR;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, t = (int)(w / chunks), row = (int)(w % chunks) * RPW + lane / LPR, d = (lane % LPR) * 8;
+    const int lane = threadIdx.x & 63, t = (int)(w / parts), row0 = (int)(w % parts) * RPW * KV_U + lane / LPR, d = (lane % LPR) * 8;
     if (t >= a.n_rows) return;
     bool padding;
     const KvSlot s = kv_slot(a, t, lane, padding);
-    if (padding || row >= 2 * a.c.kv_heads) return;
-    const bool value = row >= a.c.kv_heads;
-    const int head = value ? row - a.c.kv_heads : row;
+    if (padding) return;
     typedef typename Store<ACT>::type act_t;
     typedef typename Store<ST>::type st_t;
-    act_t *dst = (act_t *)(value ? a.v : a.k) + t * (value ? a.v_stride : a.k_stride) + head * HD + d;
-    float x[8];
-    if (s.in) {
-        const st_t *src = (const st_t *)(value ? a.c.v : a.c.k) + s.row + (int64_t)head * a.c.page * HD + d;
-        if constexpr (ST == ACT) {
-            store_raw8<ACT>(dst, load_raw8<ACT>(src));
-            return;
-        } else {
-            load8<ST>(src, x);
-            const float scale = (value ? a.c.v_scale : a.c.k_scale)[s.scale + (int64_t)head * a.c.page];
+    Raw8<ST == ACT ? ACT : HIPVOC_T_BF16> raw[KV_U];
+    u32x2 codes[KV_U];
+    float scale[KV_U];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= scale;
+    for (int u = 0; u < KV_U; u++) {
+        const int row = row0 + u * RPW, value = row >= a.c.kv_heads, head = value ? row - a.c.kv_heads : row;
+        if (row < 2 * a.c.kv_heads && s.in) {
+            const st_t *src = (const st_t *)(value ? a.c.v : a.c.k) + s.row + (int64_t)head * a.c.page * HD + d;
+            if constexpr (ST == ACT) {
+                raw[u] = load_raw8<ACT>(src);
+            } else {
+                codes[u] = *(const u32x2 *)src;
+                scale[u] = (value ? a.c.v_scale : a.c.k_scale)[s.scale + (int64_t)head * a.c.page];
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __builtin_nanf("");
     }
-    store8<ACT>(dst, x);
+#pragma unroll
+    for (int u = 0; u < KV_U; u++) {
+        const int row = row0 + u * RPW, value = row >= a.c.kv_heads, head = value ? row - a.c.kv_heads : row;
+        if (row >= 2 * a.c.kv_heads) continue;
+        act_t *dst = (act_t *)(value ? a.v : a.k) + t * (value ? a.v_stride : a.k_stride) + head * HD + d;
+        float x[8];
+        if (s.in) {
+            if constexpr (ST == ACT) {
+                store_raw8<ACT>(dst, raw[u]);
+                continue;
+            } else {
+                load8<ST>(&codes[u], x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] *= scale[u];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __builtin_nanf("");
+        }
+        store8<ACT>(dst, x);
+    }
 }
 
 template <int ACT, int ST, int HD> static hipError_t kv_go(const KvMoveArgs &a, bool write, hipStream_t s) {
-    constexpr int RPW = 64 / (HD / 8);
-    const int chunks = (2 * a.c.kv_heads + RPW - 1) / RPW;
-    const int64_t blocks = ((int64_t)a.n_rows * chunks + 3) / 4;
+    constexpr int per = 64 / (HD / 8) * KV_U;
+    const int parts = (2 * a.c.kv_heads + per - 1) / per;
+    const int64_t blocks = ((int64_t)a.n_rows * parts + 3) / 4;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    if (write) kv_write_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, chunks);
-    else kv_read_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, chunks);
+    if (write) kv_write_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, parts);
+    else kv_read_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, parts);
     return hipGetLastError();
 }
 template <int ACT, int ST> static hipError_t kv_hd(const KvMoveArgs &a, bool write, hipStream_t s) {

@@ -3,20 +3,19 @@
 // Mathematics: s = x + r, y = s / sqrt(mean s^2 + eps) * w; 8 bits: y ~ code * (max|y| / TOP) per group of columns.  Everything in 32
 // bits; s is rounded once where it is stored, y once (or to a code).
 // Bound: memory (and, for a few rows, the latency of one load, one reduction and one store).  A row is read once and stays in
-// registers: NV vectors of eight values per thread, TH threads per row; rows of up to 64 * 8 * 4 values are a wave's own, four rows to a
-// workgroup, so the usual reduction is a butterfly without a barrier.
+// registers: NV vectors of eight values per thread, TH threads per row; rows of up to 1024 values are a wave's own, four rows to a workgroup
+// (no barrier); 2048 values: 256 threads and one vector each beat a wave with four (8192 rows to e4m3: 26.5 against 28.2 us).
 #include "ops_device.h"
 
 namespace hipvoc {
 
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ float wave_amax(float v, int width = 64) {
-    for (int o = 1; o < width; o *= 2) v = amax_nan(v, __shfl_xor(v, o));
-    return v;
+    v += __uint_as_float(dpp<0xb1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x4e>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
 }
 
 // OUT == ACT: y in the act type, else codes.  TH threads (64, 256 or 1024) have a row; a workgroup has max(TH, 256) threads.
@@ -24,7 +23,8 @@ template <int ACT, int OUT, int TH, int NV>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormArgs a) {
     constexpr int ROWS = TH < 256 ? 256 / TH : 1, NWAVE = TH / 64;
     typedef typename Store<ACT>::type act_t;
-    __shared__ float sh[2][NWAVE > 1 ? NWAVE : 1];
+    __shared__ float sh[NWAVE > 1 ? NWAVE : 1];
+    __shared__ unsigned sh_top[NWAVE > 1 ? NWAVE : 1];
     const int t = threadIdx.x % TH, row = blockIdx.x * ROWS + threadIdx.x / TH, vecs = a.cols / 8;
     if (ROWS > 1 && row >= a.rows) return;                      // a wave's own row: no barrier follows
     const act_t *x = (const act_t *)a.x + row * a.x_stride, *r = (const act_t *)a.residual + row * a.residual_stride;
@@ -59,14 +59,14 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
     }
     sq = wave_sum(sq);
     if constexpr (NWAVE > 1) {
-        if ((t & 63) == 0) sh[0][t >> 6] = sq;
+        if ((t & 63) == 0) sh[t >> 6] = sq;
         __syncthreads();
         sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < NWAVE; i++) sq += sh[0][i];
+        for (int i = 0; i < NWAVE; i++) sq += sh[i];
     }
     const float rs = 1.f / sqrtf(sq / (float)a.cols + a.eps);
-    float top = 0.f;
+    unsigned top = 0;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         const int i = v * TH + t;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             s[v][e] = s[v][e] * rs * w[v][e];
-            if constexpr (OUT != ACT) top = amax_nan(top, s[v][e]);
+            if constexpr (OUT != ACT) top = amax_bits(top, s[v][e]);
         }
         if constexpr (OUT == ACT) {
             if (i < vecs) store8<ACT>((act_t *)a.y + row * a.y_stride + i * 8, s[v]);
@@ -83,19 +83,20 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
     if constexpr (OUT != ACT) {
         uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
         if (a.group == 0) {
-            top = wave_amax(top);
+            top = amax_wave(top);
             if constexpr (NWAVE > 1) {
-                if ((t & 63) == 0) sh[1][t >> 6] = top;
+                if ((t & 63) == 0) sh_top[t >> 6] = top;
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < NWAVE; i++) top = amax_nan(top, sh[1][i]);
+                for (int i = 0; i < NWAVE; i++) top = max(top, sh_top[i]);
             }
-            const float scale = scale8<OUT>(top);
+            const float scale = scale8<OUT>(__uint_as_float(top));
+            const Coder<OUT> code(scale);
             if (t == 0) a.scales[row] = scale;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int i = v * TH + t;
-                if (i < vecs) *(u32x2 *)(y + i * 8) = codes8<OUT>(s[v], scale);
+                if (i < vecs) *(u32x2 *)(y + i * 8) = code.eight(s[v]);
             }
         } else {
             // a group is 4, 8 or 16 neighbouring lanes of one vector index (TH is a multiple of 16)
@@ -103,12 +104,12 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
 #pragma unroll
             for (int v = 0; v < NV; v++) {
                 const int i = v * TH + t;
-                float g = 0.f;
+                unsigned g = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) g = amax_nan(g, s[v][e]);
-                const float scale = scale8<OUT>(wave_amax(g, lanes));
+                for (int e = 0; e < 8; e++) g = amax_bits(g, s[v][e]);
+                const float scale = scale8<OUT>(__uint_as_float(amax_lanes(g, lanes)));
                 if (i < vecs) {
-                    *(u32x2 *)(y + i * 8) = codes8<OUT>(s[v], scale);
+                    *(u32x2 *)(y + i * 8) = Coder<OUT>(scale).eight(s[v]);
                     if (i % lanes == 0) a.scales[(int64_t)row * (a.cols / a.group) + i / lanes] = scale;
                 }
             }
@@ -147,11 +148,12 @@ __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(NormArgs a) {
         // a group per wave; the whole row: all four waves find the same maximum over all of it, and each codes a quarter
         const bool whole = a.group == 0;
         for (int g = whole ? 0 : t >> 6; g < groups; g += 4) {
-            float top = 0.f;
-            for (int i = lane; i < n; i += 64) top = amax_nan(top, y_of(g * n + i));
-            const float scale = scale8<OUT>(wave_amax(top));
+            unsigned top = 0;
+            for (int i = lane; i < n; i += 64) top = amax_bits(top, y_of(g * n + i));
+            const float scale = scale8<OUT>(__uint_as_float(amax_wave(top)));
+            const Coder<OUT> code(scale);
             if (lane == 0 && (!whole || t == 0)) a.scales[(int64_t)row * groups + g] = scale;
-            for (int i = whole ? t : lane; i < n; i += whole ? 256 : 64) y[g * n + i] = code1<OUT>(y_of(g * n + i), scale);
+            for (int i = whole ? t : lane; i < n; i += whole ? 256 : 64) y[g * n + i] = code.one(y_of(g * n + i));
         }
         __syncthreads();
         if (a.sum)
@@ -173,7 +175,7 @@ template <int ACT, int OUT> static hipError_t norm_out(const NormArgs &a, hipStr
     if (any || vecs > 4096) add_rmsnorm_any_kernel<ACT, OUT><<<a.rows, 256, 0, s>>>(a);
     else if (vecs <= 64) norm_go<ACT, OUT, 64, 1>(a, s);
     else if (vecs <= 128) norm_go<ACT, OUT, 64, 2>(a, s);
-    else if (vecs <= 256) norm_go<ACT, OUT, 64, 4>(a, s);
+    else if (vecs <= 256) norm_go<ACT, OUT, 256, 1>(a, s);
     else if (vecs <= 512) norm_go<ACT, OUT, 256, 2>(a, s);
     else if (vecs <= 1024) norm_go<ACT, OUT, 256, 4>(a, s);
     else norm_go<ACT, OUT, 1024, 4>(a, s);

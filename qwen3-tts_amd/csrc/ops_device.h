@@ -102,40 +102,80 @@ template <int T> __device__ __forceinline__ float scale8(float amax) {
     constexpr float inv = 1.0f / (T == HIPVOC_T_INT8 ? 127.f : 448.f);
     return amax * inv;
 }
-// max|x| that keeps NaN (fmaxf would drop it): a row with a NaN gets scale NaN, one with an infinity scale infinity, and both read back as NaN
-__device__ __forceinline__ float amax_nan(float m, float x) {
-    const float a = fabsf(x);
-    return (a > m || a != a) ? a : m;      // m NaN: a > NaN is false, m stays unless a is NaN as well
+// max|x| that keeps NaN (fmaxf would drop it): magnitudes compare like their bits, a NaN above an infinity.  A row with a NaN gets scale NaN, one with
+// an infinity scale infinity, and both read back as NaN.
+__device__ __forceinline__ unsigned amax_bits(unsigned m, float x) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+// ... over 4, 8 or 16 neighbouring lanes (quad permutations, then mirrors of 8 and 16: what is left of a mirror is alike in all its lanes), or the wave
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+__device__ __forceinline__ unsigned amax_lanes(unsigned m, int lanes) {
+    m = max(m, dpp<0xb1>(m));
+    m = max(m, dpp<0x4e>(m));
+    if (lanes > 4) m = max(m, dpp<0x141>(m));
+    if (lanes > 8) m = max(m, dpp<0x140>(m));
+    return m;
 }
-template <int T> __device__ __forceinline__ float code_quotient(float x, float scale) {
-    const float t = scale > 0.f && scale < __builtin_inff() ? x / scale : 0.f;      // infinite or NaN scale: code 0, which reads back as NaN
-    return fminf(fmaxf(t, -top8<T>()), top8<T>());
+__device__ __forceinline__ unsigned amax_wave(unsigned m) {
+    m = amax_lanes(m, 16);
+    m = max(m, (unsigned)__shfl_xor((int)m, 16));
+    return max(m, (unsigned)__shfl_xor((int)m, 32));
 }
-template <int T> __device__ __forceinline__ u32x2 codes8(const float *x, float scale) {
-    float t[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) t[i] = code_quotient<T>(x[i], scale);
-    u32x2 r;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if constexpr (T == HIPVOC_T_INT8) {
-            unsigned u = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) u |= ((unsigned)(int)rintf(t[4 * h + i]) & 0xffu) << (8 * i);
-            r[h] = u;
-        } else {
-            int u = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h], t[4 * h + 1], 0, false);
-            u = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h + 2], t[4 * h + 3], u, true);
-            r[h] = (unsigned)u;
-        }
+
+// x / scale, correctly rounded, for many x: with y = 1 / scale correctly rounded, q = x y is within an ulp or two of the quotient, x - q scale is exact in
+// one fused step and q + (x - q scale) y is the quotient rounded once (Markstein 1990), three instructions for a dozen.  It needs room below x
+// for the remainder, so small scales take the division.  scale 0, infinite or NaN: 0, which reads back as 0 or NaN.
+template <int T> struct Coder {
+    float scale, inv;
+    bool fast;
+    __device__ __forceinline__ explicit Coder(float s) : scale(s) {
+        fast = s > 0x1p-80f && s < 0x1p+80f;
+        inv = 1.f / (fast ? s : 1.f);
     }
-    return r;
-}
-template <int T> __device__ __forceinline__ uint8_t code1(float x, float scale) {
-    const float t = code_quotient<T>(x, scale);
-    if constexpr (T == HIPVOC_T_INT8) return (uint8_t)(int)rintf(t);
-    else return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false) & 0xff);
-}
+    __device__ __forceinline__ float quotient(float x) const {
+        float t;
+        if (fast) {
+            const float q = x * inv;
+            t = fmaf(fmaf(-q, scale, x), inv, q);
+        } else {
+            t = scale > 0.f && scale < __builtin_inff() ? x / scale : 0.f;
+        }
+        return fminf(fmaxf(t, -top8<T>()), top8<T>());
+    }
+    __device__ __forceinline__ u32x2 eight(const float *x) const {
+        float t[8];
+        if (fast) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float q = x[i] * inv;
+                t[i] = fmaf(fmaf(-q, scale, x[i]), inv, q);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) t[i] = quotient(x[i]);
+        }
+        u32x2 r;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[4 * h + i] = __builtin_amdgcn_fmed3f(t[4 * h + i], -top8<T>(), top8<T>());
+            if constexpr (T == HIPVOC_T_INT8) {
+                unsigned u = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) u |= ((unsigned)(int)rintf(t[4 * h + i]) & 0xffu) << (8 * i);
+                r[h] = u;
+            } else {
+                int u = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h], t[4 * h + 1], 0, false);
+                u = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * h + 2], t[4 * h + 3], u, true);
+                r[h] = (unsigned)u;
+            }
+        }
+        return r;
+    }
+    __device__ __forceinline__ uint8_t one(float x) const {
+        const float t = quotient(x);
+        if constexpr (T == HIPVOC_T_INT8) return (uint8_t)(int)rintf(t);
+        else return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false) & 0xff);
+    }
+};
 
 __device__ __forceinline__ void raise(int *err, int bit) { atomicOr(err, bit); }
 
