@@ -198,20 +198,19 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
                 float x = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) x = fmaf(q[h][i], k[u][i], x);
-#pragma unroll
-                for (int off = 1; off < LPR; off *= 2) x += __shfl_xor(x, off);
+                x = sum_lanes<LPR>(x);
                 if constexpr (ST != ACT) x *= ks[u];
                 s[h][u] = in[u] ? x * a.scale_log2 : -__builtin_inff();
                 top = fmaxf(top, s[h][u]);
             }
-            const float safe = top == -__builtin_inff() ? 0.f : top, old = exp2f(m[h] - safe);
+            const float safe = top == -__builtin_inff() ? 0.f : top, old = __builtin_amdgcn_exp2f(m[h] - safe);
             m[h] = top;
             l[h] *= old;
 #pragma unroll
             for (int i = 0; i < 8; i++) o[h][i] *= old;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                float p = exp2f(s[h][u] - safe);
+                float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
                 l[h] += p;
                 if constexpr (ST != ACT) p = in[u] ? p * vs[u] : 0.f;
 #pragma unroll

@@ -10,10 +10,7 @@
 namespace hipvoc {
 
 __device__ __forceinline__ float wave_sum(float v) {
-    v += __uint_as_float(dpp<0xb1>(__float_as_uint(v)));
-    v += __uint_as_float(dpp<0x4e>(__float_as_uint(v)));
-    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
-    v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    v = sum_lanes<16>(v);
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }

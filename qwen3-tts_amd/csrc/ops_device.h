@@ -114,6 +114,13 @@ __device__ __forceinline__ unsigned amax_lanes(unsigned m, int lanes) {
     if (lanes > 8) m = max(m, dpp<0x140>(m));
     return m;
 }
+template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {          // LANES = 8 or 16
+    v += __uint_as_float(dpp<0xb1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x4e>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    if (LANES > 8) v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    return v;
+}
 __device__ __forceinline__ unsigned amax_wave(unsigned m) {
     m = amax_lanes(m, 16);
     m = max(m, (unsigned)__shfl_xor((int)m, 16));
