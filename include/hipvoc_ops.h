@@ -93,7 +93,8 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
  * q, out: act type, row b at b*q_stride / b*out_stride, [n_heads][head_dim]; lse [n_seqs][n_heads] f32 or NULL.
  * max_len: no lens[b] is larger (a larger one is a deferred error); the host cuts the length into parts by it, so a
  * tight bound costs least.  At most table_width * page.
- * Weights p are rounded to 16 bits for the product with V where act has 16 bits (the type of V, bf16 for 8-bit caches).
+ * Where act has 16 bits the weights p enter the product with V with 11 bits (an f16 cache) or 16 (any other); scores, sums and the
+ * product itself are in 32 bits.
  * workspace: hipvoc_attention_workspace() bytes (it may be 0), 16-byte aligned, not used by another call in flight.
  */
 size_t hipvoc_attention_workspace(const hipvoc_kv_cache *cache, int n_heads, int n_seqs, int max_len, int window);

@@ -255,8 +255,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 //   O^T = V^T P^T (rows = values' columns, columns = heads): and these, rounded, are at once the right operand.  The left one needs a column
 //                 of V for eight keys: the lane reads HD/16 neighbouring columns of its eight keys' rows (whole rows across 16 lanes) and
 //                 turns them with one byte permutation per two values; row m of product i is column m HD/16 + i.
-// So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P is rounded to 16 bits for the product with V (V's own type,
-// bf16 for 8-bit codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P).
+// So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P goes into the product with V in V's own type (bf16 for 8-bit
+// codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().
 // What is masked is read from a row that is not (so that no stale value, NaN or page number behind the last token matters).
 
 // four codes to two pairs of 16-bit values, exactly
@@ -413,8 +413,11 @@ template <int ACT, int ST, int HD> struct AttnWave {
             }
         }
     }
-    // the running maximum and sum, and the weights as the right operand of the product with V
-    __device__ __forceinline__ u32x4 weights(const Tile &tl, const float (&s)[8], int lane) {
+    // The running maximum and sum, and the weights as the right operand of the product with V: P operands whose sum they are.  One f16 (11 bits)
+    // for f16 values; else bf16 twice, what the first leaves over in the second: one bf16 alone (8 bits) would add as much error again as the
+    // rounding of the result, and the second product costs a tile 8 matrix instructions of 16 cycles and 20 vector ones, under the time of its loads.
+    static constexpr int P = PF16 ? 1 : 2;
+    __device__ __forceinline__ void weights(const Tile &tl, const float (&s)[8], int lane, u32x4 (&pp)[P]) {
         const int j = lane >> 4;
         float top = m;
 #pragma unroll
@@ -444,12 +447,17 @@ template <int ACT, int ST, int HD> struct AttnWave {
                 }
             }
         }
-        u32x4 pp;
 #pragma unroll
-        for (int e = 0; e < 4; e++) pp[e] = PF16 ? pack_f16(p[2 * e], p[2 * e + 1]) : pack_bf16(p[2 * e], p[2 * e + 1]);
-        return pp;
+        for (int e = 0; e < 4; e++) {
+            if constexpr (PF16) {
+                pp[0][e] = pack_f16(p[2 * e], p[2 * e + 1]);
+            } else {
+                pp[0][e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+                pp[P - 1][e] = pack_bf16(p[2 * e] - bf16_lo(pp[0][e]), p[2 * e + 1] - bf16_hi(pp[0][e]));
+            }
+        }
     }
-    __device__ __forceinline__ void values(u32x4 pp) {
+    __device__ __forceinline__ void values(const u32x4 (&pp)[P]) {
         unsigned w[8][HD / 32];                                          // the value rows in 16 bits
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -469,7 +477,8 @@ template <int ACT, int ST, int HD> struct AttnWave {
             u32x4 col;
 #pragma unroll
             for (int e = 0; e < 4; e++) col[e] = __builtin_amdgcn_perm(w[2 * e + 1][i >> 1], w[2 * e][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
-            o[i] = mfma32<PF16>(col, pp, o[i]);
+#pragma unroll
+            for (int p = 0; p < P; p++) o[i] = mfma32<PF16>(col, pp[p], o[i]);
         }
     }
     __device__ __forceinline__ float sum_of_head() const {
@@ -501,7 +510,9 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_whole_kernel(AttnArgs a) {
         w.load_v(a, t, pv, true, lane);
         float s[8];
         w.scores(a, t, s, lane);
-        w.values(w.weights(t, s, lane));
+        u32x4 pp[Wave::P];
+        w.weights(t, s, lane, pp);
+        w.values(pp);
     }
     const float l = w.sum_of_head();
     const bool wave_bad = __any(bad);
@@ -604,7 +615,9 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_stream_kernel(AttnArgs a) 
         float s[8];
         w.scores(a, cur.t, s, lane);
         w.load_k(a, next.t, sk, sv, left > 1, lane);
-        w.values(w.weights(cur.t, s, lane));
+        u32x4 pp[Wave::P];
+        w.weights(cur.t, s, lane, pp);
+        w.values(pp);
         w.load_v(a, next.t, sv, left > 1, lane);
         left--;
         if (left == 0 || next.tile == 0) {                               // the piece ends

@@ -103,7 +103,8 @@ def attention_ref(P, q, scale, window):
     b, heads, hd = q.shape
     outs, lses, bo, bl = [], [], [], []
     rep = heads // P.kv
-    p16 = 0.0 if P.act == torch.float32 else u(torch.bfloat16 if P.store != "same" else P.act)        # the weights' rounding for the product with V
+    # the weights' rounding for the product with V: one f16, or two bf16, the second holding what the first leaves over
+    p16 = 0.0 if P.act == torch.float32 else u(torch.float16) if P.act == torch.float16 and P.store == "same" else u(torch.bfloat16) ** 2
     for s in range(b):
         n = P.lens[s]
         lo = max(0, n - window) if window else 0
@@ -123,9 +124,9 @@ def attention_ref(P, q, scale, window):
         wv = (w[..., None] * v.abs()).sum(1)
         m = n - lo
         err = wv * (2 * delta[:, None] + p16 + (2 * m + 16) * U32)
-        if p16 and P.act == torch.float16:
+        if P.act == torch.float16 and P.store == "same":
             # weights below the type's normal range (of the largest weight, 1 before normalisation) are off by half its smallest step
-            err = err + w.amax(-1)[:, None] * m * (2.0 ** -25 if P.store == "same" else 0.0) * v.abs().amax(1)
+            err = err + w.amax(-1)[:, None] * m * 2.0 ** -25 * v.abs().amax(1)
         outs.append(out)
         bo.append(err + u(P.act) * (out.abs() + err) + 2.0 ** -24 * (P.act == torch.float16))
         lse = torch.logsumexp(score, -1)
