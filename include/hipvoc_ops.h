@@ -8,13 +8,14 @@
  * with the residual's addition (and 8-bit rows), and products with 4-bit weights.
  *
  * Conventions are hipvoc.h's: opaque handle, int 0 / negative HIPVOC_E_* codes, text in hipvoc_last_error(h), no
- * exception or abort across the boundary, calls on one handle serialised by the caller (what they enqueue may overlap:
- * a handle keeps no workspace), released with hipvoc_free().  Different from hipvoc.h: every call names the stream it is
- * enqueued on (`stream`: a hipStream_t of the handle's device, NULL = the null stream), since these operators are parts
- * of the caller's own step.  All tensors are DEVICE memory of the handle's device; they are read and written when the
- * stream gets there.  No call allocates, synchronises (but for hipvoc_ops_sync / hipvoc_sync) or changes the calling
- * thread's current device, so all of them can be captured into a HIP graph; every kernel writes all it reads back, so two
- * graphs share nothing that they are not given both.
+ * exception or abort across the boundary, released with hipvoc_free().  Different from hipvoc.h: calls on one handle may
+ * come from several threads at once (a handle keeps no workspace; the text is that of its last failure, whichever
+ * thread's), and every call names the stream it is enqueued on (`stream`: a hipStream_t of the handle's device, NULL = the
+ * null stream), since these operators are parts of the caller's own step.  All tensors are DEVICE memory of the handle's
+ * device; they are read and written when the stream gets there.  No call allocates, synchronises (but for hipvoc_ops_sync /
+ * hipvoc_sync) or changes the calling thread's current device, so all of them can be captured into a HIP graph (which must
+ * not outlive the handle: the kernels report into it); every kernel writes all it reads back, so two graphs share nothing
+ * that they are not given both.  A call whose threads do not count in 32 bits is refused.
  *
  * Deferred errors: what only the device sees (a page number, a length or an offset out of range) is never followed out of
  * bounds.  The kernel records it in the handle, leaves such a row of the cache unwritten, fills such a row of an output
@@ -93,8 +94,9 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
  * q, out: act type, row b at b*q_stride / b*out_stride, [n_heads][head_dim]; lse [n_seqs][n_heads] f32 or NULL.
  * max_len: no lens[b] is larger (a larger one is a deferred error); the host cuts the length into parts by it, so a
  * tight bound costs least.  At most table_width * page.
- * Where act has 16 bits the weights p enter the product with V with 11 bits (an f16 cache) or 16 (any other); scores, sums and the
- * product itself are in 32 bits.
+ * Where act has 16 bits the weights p enter the product with V as the sum of two f16 (an f16 cache) or two bf16 (any other), so an
+ * infinity among the values that are seen gives NaN; scores, sums and the product itself are in 32 bits.
+ * How a sequence is cut, and with it the order of its sums, depends on all lengths of the call; the same call gives the same bits.
  * workspace: hipvoc_attention_workspace() bytes (it may be 0), 16-byte aligned, not used by another call in flight.
  */
 size_t hipvoc_attention_workspace(const hipvoc_kv_cache *cache, int n_heads, int n_seqs, int max_len, int window);
@@ -106,10 +108,10 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
 /*
  * s = x + residual (in 32 bits; residual NULL: s = x), y = s / sqrt(mean(s^2) + eps) * weight, per row of `cols` values.
  * sum (act type; NULL: not wanted, and without a residual it has to be NULL) gets s rounded; y is made from s before that
- * rounding.  sum may be x or residual themselves (same stride).
+ * rounding.  sum may be x or residual themselves (same stride); y overlaps no input and not sum.
  * out_dtype = dtype: y [rows][cols] in the act type.  INT8 / E4M3: y holds codes (bytes) and scales [rows][cols/group] f32,
  * one per `group` columns (32, 64, 128, or 0 for one per row; group divides cols), code and scale as in the cache.
- * Any cols from 1 to 2^20, any alignment: rows that are no multiple of 8 long or not 16-byte aligned take a slower kernel.
+ * Fewer than 2^22 rows; any cols from 1 to 2^20, any alignment: rows that are no multiple of 8 long or not 16-byte aligned take a slower kernel.
  */
 int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
                        const void *weight, void *sum, int64_t sum_stride, void *y, int64_t y_stride, float *scales,
@@ -123,6 +125,8 @@ int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *res
  * x: row m at m*x_stride, act type, or INT8 with x_scale [n_rows][x_groups] f32 (x_groups = n_in/group, or 1 for one
  * scale per row).  y: act type y_dtype at m*y_stride; for x of an act type y_dtype is that type.
  * Every product is exact; sums of a group, and of groups, are kept in 32 bits (8-bit rows: a group's sum is an integer).
+ * Codes enter with 16 added that is taken off the sum, so a row of x that holds an infinity or NaN gives NaN, and one whose
+ * sum of |x| * scale is within a factor of 31 of the largest 32-bit number may.
  * Any n_rows: the weights are read once for every 16.  x_stride is a multiple of 16 bytes.
  */
 int hipvoc_q4_matvec(void *h, const uint8_t *codes, const void *scales, const void *mins, int n_out, int n_in, int group,

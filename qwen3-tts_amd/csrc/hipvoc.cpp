@@ -36,6 +36,8 @@ namespace hipvoc {
 // text of the calling thread's last failed hipvoc_load / hipvoc_enc_load (hipvoc_last_error(NULL)): per thread, so
 // concurrent loads (hipvoc-worker loads contexts x devices) cannot clobber or race on each other's message
 static thread_local std::string g_load_err;
+// operator handles take calls from several threads: their text is written under this, and read as a copy of the reader's own
+static std::mutex g_ops_text;
 
 static std::string fmt(const char *f, ...) {
     char buf[512];
@@ -1615,7 +1617,11 @@ template <typename Body>
 static inline int guarded(void *h, Body &&body) noexcept {
     return abi_guard(body, [h](const char *what) noexcept {
         try {
-            if (h) static_cast<Ctx *>(h)->err = what;
+            if (!h) return;
+            Ctx *c = static_cast<Ctx *>(h);
+            std::unique_lock<std::mutex> lock(g_ops_text, std::defer_lock);
+            if (c->is_ops) lock.lock();
+            c->err = what;
         } catch (...) {
         }
     });
@@ -1910,7 +1916,16 @@ const char *hipvoc_last_error(void *h) {
         // threads load or fail meanwhile
         return g_load_err.c_str();
     }
-    return ((Ctx *)h)->err.c_str();
+    Ctx *c = (Ctx *)h;
+    if (!c->is_ops) return c->err.c_str();
+    static thread_local std::string copy;
+    try {
+        std::lock_guard<std::mutex> lock(g_ops_text);
+        copy = c->err;
+    } catch (...) {
+        return "out of host memory";
+    }
+    return copy.c_str();
 }
 
 void hipvoc_free(void *h) {

@@ -2,10 +2,14 @@
 //
 // Mathematics: one pass over the keys with a running maximum m and sum l per query head (softmax in powers of two, s = q.k * scale *
 // log2(e)):  m' = max(m, s), l' = l 2^(m-m') + 2^(s-m'), o' = o 2^(m-m') + 2^(s-m') v.  States (m, l, o) of disjoint key sets join by
-// the same rule, so a sequence is cut into chunks, one workgroup each; the chunks of a sequence are joined by a second small kernel
-// (no atomics: the order of every sum is fixed).
-// Bound: memory.  Every key and value row is read once for all query heads of its key head; the split exists because n_seqs * kv_heads
-// workgroups do not fill 256 CUs.
+// the same rule.
+// Bound: memory.  Every key and value row is read once for all query heads of its key head (16 of them; 4 for 32-bit activations).
+// Split: n_seqs * kv_heads workgroups do not fill 256 CUs, and sequences differ in length.  So all the tiles of a call stand in one row and
+// every wave (32-bit activations: workgroup) has an equal share of it, wherever its ends fall (ops_index.hpp); the pieces of a sequence are
+// joined by a second kernel, without atomics: the order of every sum follows from the call's lengths.  Against a grid of fixed chunks: 128
+// sequences of 400 .. 2048 tokens in bf16 56.6 us (72), since the chip's dies got unequal chunks.  Up to 24 tiles (768 keys) a workgroup has a
+// sequence and key head to itself: 500 keys 10 us, cut 14.  8 KV heads, 128 values: 32768 tokens x 4 in bf16, 537 MB, 97 us (5.5 TB/s); in
+// 8 bits, 65536 tokens x 4, 566 MB, 110 us (5.1 TB/s).  32-bit activations: 544 MB of 32-bit cache 109 us, 272 MB of 8-bit cache 71 us.
 #include "ops_device.h"
 
 namespace hipvoc {
@@ -157,94 +161,94 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     __shared__ int sh_bad[NW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = (lane % LPR) * 8, kl = lane / LPR;
     attn_pieces<HT>(a, [&](const AttnPiece &sp) {
-    const int seq = sp.seq, kvh = sp.kvh, h0 = sp.h0, nh = min(HT, (kvh + 1) * a.group - h0);
-    if (sp.bad && threadIdx.x == 0) raise(a.err, OPS_ERR_LENGTH);
-    float q[HT][8], o[HT][8], m[HT], l[HT];
-#pragma unroll
-    for (int h = 0; h < HT; h++) {
-        m[h] = -__builtin_inff();
-        l[h] = 0.f;
-        load8<ACT>((const act_t *)a.q + seq * a.q_stride + (int64_t)min(h0 + h, h0 + nh - 1) * HD + d, q[h]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[h][i] = 0.f;
-    }
-    const int32_t *table = a.table + seq * a.table_stride;
-    bool bad = false;
-    for (int base = sp.from + wave * TILE; base < sp.to; base += NW * TILE) {
-        float k[U][8], v[U][8], ks[U], vs[U], s[HT][U];
-        bool in[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int key = base + u * KPS + kl, kc = min(max(key, sp.lo), sp.to - 1);       // what is masked is read from a row that is not
-            in[u] = key >= sp.lo && key < sp.to;
-            int page = table[kc >> a.page_shift];
-            if (!page_ok(page, a.c.n_pages)) { bad = true; page = 0; }
-            const int in_page = kc & (a.c.page - 1);
-            const int64_t row = page * a.c.page_stride + ((int64_t)kvh * a.c.page + in_page) * HD + d;
-            load8<ST>((const st_t *)a.c.k + row, k[u]);
-            load8<ST>((const st_t *)a.c.v + row, v[u]);
-            ks[u] = vs[u] = 1.f;
-            if constexpr (ST != ACT) {
-                const int64_t sc = ((int64_t)page * a.c.kv_heads + kvh) * a.c.page + in_page;
-                ks[u] = a.c.k_scale[sc];
-                vs[u] = a.c.v_scale[sc];
-            }
-        }
+        const int seq = sp.seq, kvh = sp.kvh, h0 = sp.h0, nh = min(HT, (kvh + 1) * a.group - h0);
+        if (sp.bad && threadIdx.x == 0) raise(a.err, OPS_ERR_LENGTH);
+        float q[HT][8], o[HT][8], m[HT], l[HT];
 #pragma unroll
         for (int h = 0; h < HT; h++) {
-            float top = m[h];
+            m[h] = -__builtin_inff();
+            l[h] = 0.f;
+            load8<ACT>((const act_t *)a.q + seq * a.q_stride + (int64_t)min(h0 + h, h0 + nh - 1) * HD + d, q[h]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[h][i] = 0.f;
+        }
+        const int32_t *table = a.table + seq * a.table_stride;
+        bool bad = false;
+        for (int base = sp.from + wave * TILE; base < sp.to; base += NW * TILE) {
+            float k[U][8], v[U][8], ks[U], vs[U], s[HT][U];
+            bool in[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                float x = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) x = fmaf(q[h][i], k[u][i], x);
-                x = sum_lanes<LPR>(x);
-                if constexpr (ST != ACT) x *= ks[u];
-                s[h][u] = in[u] ? x * a.scale_log2 : -__builtin_inff();
-                top = fmaxf(top, s[h][u]);
+                const int key = base + u * KPS + kl, kc = min(max(key, sp.lo), sp.to - 1);       // what is masked is read from a row that is not
+                in[u] = key >= sp.lo && key < sp.to;
+                int page = table[kc >> a.page_shift];
+                if (!page_ok(page, a.c.n_pages)) { bad = true; page = 0; }
+                const int in_page = kc & (a.c.page - 1);
+                const int64_t row = page * a.c.page_stride + ((int64_t)kvh * a.c.page + in_page) * HD + d;
+                load8<ST>((const st_t *)a.c.k + row, k[u]);
+                load8<ST>((const st_t *)a.c.v + row, v[u]);
+                ks[u] = vs[u] = 1.f;
+                if constexpr (ST != ACT) {
+                    const int64_t sc = ((int64_t)page * a.c.kv_heads + kvh) * a.c.page + in_page;
+                    ks[u] = a.c.k_scale[sc];
+                    vs[u] = a.c.v_scale[sc];
+                }
             }
-            const float safe = top == -__builtin_inff() ? 0.f : top, old = __builtin_amdgcn_exp2f(m[h] - safe);
-            m[h] = top;
-            l[h] *= old;
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[h][i] *= old;
+            for (int h = 0; h < HT; h++) {
+                float top = m[h];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
-                l[h] += p;
-                if constexpr (ST != ACT) p = in[u] ? p * vs[u] : 0.f;
+                for (int u = 0; u < U; u++) {
+                    float x = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
+                    for (int i = 0; i < 8; i++) x = fmaf(q[h][i], k[u][i], x);
+                    x = sum_lanes<LPR>(x);
+                    if constexpr (ST != ACT) x *= ks[u];
+                    s[h][u] = in[u] ? x * a.scale_log2 : -__builtin_inff();
+                    top = fmaxf(top, s[h][u]);
+                }
+                const float safe = top == -__builtin_inff() ? 0.f : top, old = __builtin_amdgcn_exp2f(m[h] - safe);
+                m[h] = top;
+                l[h] *= old;
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[h][i] *= old;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
+                    l[h] += p;
+                    if constexpr (ST != ACT) p = in[u] ? p * vs[u] : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
+                }
             }
         }
-    }
-    const bool wave_bad = __any(bad);
-    if (lane == 0) {
-        if (wave_bad) raise(a.err, OPS_ERR_PAGE);
-        sh_bad[wave] = wave_bad || sp.bad;
-    }
-    // join the wave's KPS key groups, then the four waves
-#pragma unroll
-    for (int h = 0; h < HT; h++) {
-#pragma unroll
-        for (int off = LPR; off < 64; off *= 2) {
-            const float m2 = __shfl_xor(m[h], off), l2 = __shfl_xor(l[h], off), top = fmaxf(m[h], m2), safe = top == -__builtin_inff() ? 0.f : top;
-            const float f1 = exp2f(m[h] - safe), f2 = exp2f(m2 - safe);
-            m[h] = top;
-            l[h] = l[h] * f1 + l2 * f2;
-#pragma unroll
-            for (int i = 0; i < 8; i++) o[h][i] = o[h][i] * f1 + __shfl_xor(o[h][i], off) * f2;
+        const bool wave_bad = __any(bad);
+        if (lane == 0) {
+            if (wave_bad) raise(a.err, OPS_ERR_PAGE);
+            sh_bad[wave] = wave_bad || sp.bad;
         }
-        if (kl == 0) {
+        // join the wave's KPS key groups, then the four waves
 #pragma unroll
-            for (int i = 0; i < 8; i++) sh_o[wave][h][d + i] = o[h][i];
-            if (d == 0) { sh_m[wave][h] = m[h]; sh_l[wave][h] = l[h]; }
+        for (int h = 0; h < HT; h++) {
+#pragma unroll
+            for (int off = LPR; off < 64; off *= 2) {
+                const float m2 = __shfl_xor(m[h], off), l2 = __shfl_xor(l[h], off), top = fmaxf(m[h], m2), safe = top == -__builtin_inff() ? 0.f : top;
+                const float f1 = exp2f(m[h] - safe), f2 = exp2f(m2 - safe);
+                m[h] = top;
+                l[h] = l[h] * f1 + l2 * f2;
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[h][i] = o[h][i] * f1 + __shfl_xor(o[h][i], off) * f2;
+            }
+            if (kl == 0) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) sh_o[wave][h][d + i] = o[h][i];
+                if (d == 0) { sh_m[wave][h] = m[h]; sh_l[wave][h] = l[h]; }
+            }
         }
-    }
-    __syncthreads();
-    attn_finish<ACT, HD, NW, HT>(a, sp, nh, (sh_bad[0] | sh_bad[1] | sh_bad[2] | sh_bad[3]) != 0, [&](int w, int h) { return f32v2{sh_m[w][h], sh_l[w][h]}; },
-                                [&](int w, int h, int d) { return sh_o[w][h][d]; });
-    __syncthreads();                                                     // another piece may follow
+        __syncthreads();
+        attn_finish<ACT, HD, NW, HT>(a, sp, nh, (sh_bad[0] | sh_bad[1] | sh_bad[2] | sh_bad[3]) != 0, [&](int w, int h) { return f32v2{sh_m[w][h], sh_l[w][h]}; },
+                                    [&](int w, int h, int d) { return sh_o[w][h][d]; });
+        __syncthreads();                                                     // another piece may follow
     });
 }
 
@@ -255,8 +259,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 //   O^T = V^T P^T (rows = values' columns, columns = heads): and these, rounded, are at once the right operand.  The left one needs a column
 //                 of V for eight keys: the lane reads HD/16 neighbouring columns of its eight keys' rows (whole rows across 16 lanes) and
 //                 turns them with one byte permutation per two values; row m of product i is column m HD/16 + i.
-// So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P goes into the product with V in V's own type (bf16 for 8-bit
-// codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().
+// So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P goes into the product with V as two values of V's own type (bf16 for
+// 8-bit codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().
 // What is masked is read from a row that is not (so that no stale value, NaN or page number behind the last token matters).
 
 // four codes to two pairs of 16-bit values, exactly
@@ -288,15 +292,11 @@ __device__ __forceinline__ float max_of_head(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-#if !defined(ATTN_NT) || ATTN_NT
+// Keys and values are read once: non-temporal loads (512 MB: 6.9 TB/s against 6.1).
 template <typename T> __device__ __forceinline__ T once(const T *p) { return __builtin_nontemporal_load(p); }
-#else
-template <typename T> __device__ __forceinline__ T once(const T *p) { return *p; }
-#endif
 
-#ifndef ATTN_OCC
-#define ATTN_OCC 3
-#endif
+// Waves per SIMD that the matrix kernels' registers have to leave room for: up to 168, and attn_stream_kernel has 158 .. 165 for head_dim 128.
+static constexpr int ATTN_WAVES = 3;
 
 // The keys and values of one tile for one wave, and what they do to the state of its heads
 template <int ACT, int ST, int HD> struct AttnWave {
@@ -313,6 +313,11 @@ template <int ACT, int ST, int HD> struct AttnWave {
     unsigned v[8][VW];
     f32x4 ks[2], vs[2], o[NV];
     float m, l;
+
+    // The state counts in 2^SHIFT: l and o hold 2^(s - m + SHIFT).  Without it an f16 weight under 2^-14 of the largest would lose bits (and a long
+    // cache of small weights its sum); so they keep theirs down to 2^-29.
+    static constexpr float SHIFT = PF16 ? 15.f : 0.f;
+    __device__ __forceinline__ float base_of() const { return m - SHIFT; }          // what a state's sums are relative to
 
     static __device__ __forceinline__ bool whole(const Tile &t) { return t.base >= t.lo && t.base + 32 <= t.hi; }
     // group e of eight keys, or another one where all of it is masked
@@ -401,9 +406,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
                 for (int i = 0; i < NC; i++) acc = mfma32<QF16>(k[t][i], q[i], acc);
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                s[4 * t + r] = acc[r] * a.scale_log2;
-            }
+            for (int r = 0; r < 4; r++) s[4 * t + r] = acc[r] * a.scale_log2;
         }
         if (!whole(tl)) {
 #pragma unroll
@@ -413,24 +416,23 @@ template <int ACT, int ST, int HD> struct AttnWave {
             }
         }
     }
-    // The running maximum and sum, and the weights as the right operand of the product with V: P operands whose sum they are.  One f16 (11 bits)
-    // for f16 values; else bf16 twice, what the first leaves over in the second: one bf16 alone (8 bits) would add as much error again as the
-    // rounding of the result, and the second product costs a tile 8 matrix instructions of 16 cycles and 20 vector ones, under the time of its loads.
-    static constexpr int P = PF16 ? 1 : 2;
-    __device__ __forceinline__ void weights(const Tile &tl, const float (&s)[8], int lane, u32x4 (&pp)[P]) {
+    // The running maximum and sum, and the weights as the right operand of the product with V: two operands whose sum they are, in the second what
+    // the first leaves over.  One alone (bf16: 8 bits, f16: 11) would add as much error again as the rounding of the result, or a good part of it, and
+    // the second product costs a tile 8 matrix instructions of 16 cycles and 20 vector ones, under the time of its loads: no time measured.
+    __device__ __forceinline__ void weights(const Tile &tl, const float (&s)[8], int lane, u32x4 (&pp)[2]) {
         const int j = lane >> 4;
         float top = m;
 #pragma unroll
         for (int e = 0; e < 8; e++) top = fmaxf(top, s[e]);
         top = max_of_head(top);
         if (__any(top > m)) {                                            // else nothing to scale down
-            const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.f : top));
+            const float f = __builtin_amdgcn_exp2f(base_of() - (top == -__builtin_inff() ? 0.f : top - SHIFT));
             m = top;
             l *= f;
 #pragma unroll
             for (int i = 0; i < NV; i++) o[i] *= f;
         }
-        const float safe = m == -__builtin_inff() ? 0.f : m;
+        const float safe = m == -__builtin_inff() ? 0.f : base_of();
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -450,14 +452,17 @@ template <int ACT, int ST, int HD> struct AttnWave {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if constexpr (PF16) {
-                pp[0][e] = pack_f16(p[2 * e], p[2 * e + 1]);
+                const unsigned hi = pack_f16(p[2 * e], p[2 * e + 1]);
+                const h16x2 most = __builtin_bit_cast(h16x2, hi);       // (cast from pp[0][e] itself the compiler takes pp[0][0])
+                pp[0][e] = hi;
+                pp[1][e] = pack_f16(p[2 * e] - (float)most[0], p[2 * e + 1] - (float)most[1]);
             } else {
                 pp[0][e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-                pp[P - 1][e] = pack_bf16(p[2 * e] - bf16_lo(pp[0][e]), p[2 * e + 1] - bf16_hi(pp[0][e]));
+                pp[1][e] = pack_bf16(p[2 * e] - bf16_lo(pp[0][e]), p[2 * e + 1] - bf16_hi(pp[0][e]));
             }
         }
     }
-    __device__ __forceinline__ void values(const u32x4 (&pp)[P]) {
+    __device__ __forceinline__ void values(const u32x4 (&pp)[2]) {
         unsigned w[8][HD / 32];                                          // the value rows in 16 bits
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -478,7 +483,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
 #pragma unroll
             for (int e = 0; e < 4; e++) col[e] = __builtin_amdgcn_perm(w[2 * e + 1][i >> 1], w[2 * e][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
 #pragma unroll
-            for (int p = 0; p < P; p++) o[i] = mfma32<PF16>(col, pp[p], o[i]);
+            for (int p = 0; p < 2; p++) o[i] = mfma32<PF16>(col, pp[p], o[i]);
         }
     }
     __device__ __forceinline__ float sum_of_head() const {
@@ -489,7 +494,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
 
 // A workgroup per (sequence, pair), its four waves on every fourth tile
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256, ATTN_OCC) void attn_whole_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, ATTN_WAVES) void attn_whole_kernel(AttnArgs a) {
     typedef AttnWave<ACT, ST, HD> Wave;
     constexpr int NW = 4, NV = HD / 16;
     __shared__ __attribute__((aligned(16))) float sh_o[NW][16][HD + 4];
@@ -510,7 +515,7 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_whole_kernel(AttnArgs a) {
         w.load_v(a, t, pv, true, lane);
         float s[8];
         w.scores(a, t, s, lane);
-        u32x4 pp[Wave::P];
+        u32x4 pp[2];
         w.weights(t, s, lane, pp);
         w.values(pp);
     }
@@ -526,7 +531,7 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_whole_kernel(AttnArgs a) {
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int i = 0; i < NV; i += 4) *(f32x4 *)&sh_o[wave][m16][(4 * j + r) * NV + i] = (f32x4){w.o[i][r], w.o[i + 1][r], w.o[i + 2][r], w.o[i + 3][r]};
-        if (j == 0) { sh_m[wave][m16] = w.m; sh_l[wave][m16] = l; }
+        if (j == 0) { sh_m[wave][m16] = w.base_of(); sh_l[wave][m16] = l; }
     }
     __syncthreads();
     AttnPiece p = {seq, kvh, h0, sp.lo, sp.base, sp.hi, -1, sp.bad};
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_whole_kernel(AttnArgs a) {
 // their way as soon as this one's are used up, its values likewise, and the pages of the one after that; at a piece's end only the state is
 // written and the next head's q read.
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256, ATTN_OCC) void attn_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, ATTN_WAVES) void attn_stream_kernel(AttnArgs a) {
     typedef AttnWave<ACT, ST, HD> Wave;
     constexpr int NV = HD / 16;
     __shared__ int64_t before[ATTN_MAX_SEQS + 1];
@@ -615,7 +620,7 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_stream_kernel(AttnArgs a) 
         float s[8];
         w.scores(a, cur.t, s, lane);
         w.load_k(a, next.t, sk, sv, left > 1, lane);
-        u32x4 pp[Wave::P];
+        u32x4 pp[2];
         w.weights(cur.t, s, lane, pp);
         w.values(pp);
         w.load_v(a, next.t, sv, left > 1, lane);
@@ -644,7 +649,7 @@ __global__ __launch_bounds__(256, ATTN_OCC) void attn_stream_kernel(AttnArgs a) 
                     }
                 }
                 if (j == 0) {
-                    const float m = nan ? __builtin_nanf("") : w.m, ll = nan ? __builtin_nanf("") : l;
+                    const float m = nan ? __builtin_nanf("") : w.base_of(), ll = nan ? __builtin_nanf("") : l;
                     if (!all) *slot_ml<HD, 16>(a, slot, m16) = (f32v2){m, ll};
                     else if (a.lse) a.lse[(int64_t)cur.seq * a.n_heads + h0 + m16] = lse_of(m, ll);
                 }

@@ -41,9 +41,7 @@ __device__ __forceinline__ KvSlot kv_slot(const KvMoveArgs &a, int t, int lane, 
     return s;
 }
 
-// A wave takes KV_U times 64 lanes' worth of its token's rows, all their loads ahead of the question where they belong
-static constexpr int KV_U = 4;
-
+// A wave takes KV_U times 64 lanes' worth of its token's rows, all their loads ahead of the question where they belong.
 template <int ACT, int ST, int HD>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvMoveArgs a, int parts) {
     constexpr int LPR = HD / 8, RPW = 64 / LPR;
@@ -134,12 +132,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvMoveArgs a, int parts) {
 }
 
 template <int ACT, int ST, int HD> static hipError_t kv_go(const KvMoveArgs &a, bool write, hipStream_t s) {
-    constexpr int per = 64 / (HD / 8) * KV_U;
-    const int parts = (2 * a.c.kv_heads + per - 1) / per;
-    const int64_t blocks = ((int64_t)a.n_rows * parts + 3) / 4;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    if (write) kv_write_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, parts);
-    else kv_read_kernel<ACT, ST, HD><<<(unsigned)blocks, 256, 0, s>>>(a, parts);
+    const int parts = kv_parts(a.c.kv_heads, HD);
+    const unsigned blocks = (unsigned)(((int64_t)a.n_rows * parts + 3) / 4);
+    if (write) kv_write_kernel<ACT, ST, HD><<<blocks, 256, 0, s>>>(a, parts);
+    else kv_read_kernel<ACT, ST, HD><<<blocks, 256, 0, s>>>(a, parts);
     return hipGetLastError();
 }
 template <int ACT, int ST> static hipError_t kv_hd(const KvMoveArgs &a, bool write, hipStream_t s) {

@@ -98,13 +98,6 @@ template <int XT> struct XRow {
     }
 };
 
-#ifndef Q4_RTB
-#define Q4_RTB 2
-#define Q4_KWB 2
-#endif
-#ifndef Q4_WIDE
-#define Q4_WIDE 16384
-#endif
 static constexpr int Q4_WAVES = 8, Q4_HALVES = 2, Q4_GROUPS = 128;      // waves of a workgroup; of the wide kernel, on how many shares of a block's slabs; groups of a row whose scales are in LDS at a time
 
 // What a wave reads of one slab of 128 columns
@@ -261,7 +254,7 @@ __device__ __forceinline__ void q4_finish(const Q4Args &a, const f32x4 (&out)[RT
 template <int XT, bool MINS>
 __device__ __forceinline__ void q4_stage_scales(const Q4Args &a, h16x2 *scales, float (*x_scales)[16], int n0, int m0, int wg_rows, int groups, int g0, int stride) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, n = min(Q4_GROUPS, groups - g0);
-            if (groups % 8 == 0 && groups <= Q4_GROUPS) {                                 // the rows are one piece of memory: eight groups a load
+    if (groups % 8 == 0 && groups <= Q4_GROUPS) {                                 // the rows are one piece of memory: eight groups a load
         const int per_row = groups / 8, count = min(wg_rows, a.n_out - n0) * per_row, step = blockDim.x;
         const u32x4 *s = (const u32x4 *)((const _Float16 *)a.scales + (int64_t)n0 * groups), *l = (const u32x4 *)((const _Float16 *)a.mins + (int64_t)n0 * groups);
         for (int first = threadIdx.x; first < count; first += 4 * step) {
@@ -282,25 +275,26 @@ __device__ __forceinline__ void q4_stage_scales(const Q4Args &a, h16x2 *scales, 
                 }
             }
         }
-    } else
-    for (int first = wave; first < wg_rows; first += 8 * nw) {               // eight rows' loads at a time: one latency
-                _Float16 v[8][2], m[8][2];
-    #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int64_t at = (int64_t)min(n0 + first + i * nw, a.n_out - 1) * groups + g0;
-    #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int g = min(lane + 64 * h, n - 1);
-                        v[i][h] = ((const _Float16 *)a.scales)[at + g];
-                        m[i][h] = MINS ? ((const _Float16 *)a.mins)[at + g] : (_Float16)0.f;
-                    }
+    } else {
+        for (int first = wave; first < wg_rows; first += 8 * nw) {                // eight rows' loads at a time: one latency
+            _Float16 v[8][2], m[8][2];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int64_t at = (int64_t)min(n0 + first + i * nw, a.n_out - 1) * groups + g0;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int g = min(lane + 64 * h, n - 1);
+                    v[i][h] = ((const _Float16 *)a.scales)[at + g];
+                    m[i][h] = MINS ? ((const _Float16 *)a.mins)[at + g] : (_Float16)0.f;
                 }
-    #pragma unroll
-                for (int i = 0; i < 8; i++)
-    #pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (first + i * nw < wg_rows && lane + 64 * h < n) scales[(first + i * nw) * stride + lane + 64 * h] = (h16x2){v[i][h], m[i][h]};
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (first + i * nw < wg_rows && lane + 64 * h < n) scales[(first + i * nw) * stride + lane + 64 * h] = (h16x2){v[i][h], m[i][h]};
+        }
+    }
     if constexpr (XT == HIPVOC_T_INT8) {
         if (a.x_groups > 1)
             for (int row = wave; row < 16; row += nw) {
@@ -419,16 +413,20 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void q4_wide_kernel(Q4Args a) {
     q4_finish<XT, RT>(a, out, red, kw, part, row0, wg_rows, n0, m0);
 }
 
+template <int XT> static size_t q4_wide_lds(int rt, int groups) {
+    return (XT == HIPVOC_T_F32 ? 24576 : XT == HIPVOC_T_INT8 ? 16384 : 32768) + q4_lds(XT == HIPVOC_T_INT8, 16 * rt * Q4_WAVES / Q4_HALVES, groups, Q4_HALVES);
+}
+static constexpr size_t Q4_LDS = 160 * 1024;
 template <int XT, int G, bool MINS, int RT> static hipError_t q4_wide(const Q4Args &a, hipStream_t s) {
     constexpr int rows = 16 * RT * Q4_WAVES / Q4_HALVES;
-    const size_t x = XT == HIPVOC_T_F32 ? 24576 : XT == HIPVOC_T_INT8 ? 16384 : 32768, lds = x + q4_lds(XT == HIPVOC_T_INT8, rows, a.n_in / G, Q4_HALVES);
+    const size_t lds = q4_wide_lds<XT>(RT, a.n_in / G);
     const auto kernel = q4_wide_kernel<XT, G, MINS, RT>;
     if (lds > 65536) {                                                            // over the default of a launch: said once per device
         static std::atomic<bool> said[64];
         int dev = 0;
         hipError_t e = hipGetDevice(&dev);
         if (e == hipSuccess && (dev >= 64 || !said[dev].load())) {
-            e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Q4_LDS);
             if (e == hipSuccess && dev < 64) said[dev] = true;
         }
         if (e != hipSuccess) return e;
@@ -453,7 +451,8 @@ template <int XT, int G, bool MINS> static hipError_t q4_rt(const Q4Args &a, hip
         if (a.n_out >= 32768) return q4_wide<XT, G, MINS, 2>(a, s);
         if (a.n_out >= 8192) return direct(2, q4_kernel<XT, G, MINS, 2>);
     } else {
-        if (a.n_out >= 65536) return q4_wide<XT, G, MINS, 4>(a, s);
+        // 16-bit rows of over 126 groups: their scales and x do not fit the LDS beside each other with 256 rows
+        if (a.n_out >= 65536 && q4_wide_lds<XT>(4, a.n_in / G) <= Q4_LDS) return q4_wide<XT, G, MINS, 4>(a, s);
         if (a.n_out >= 16384) return q4_wide<XT, G, MINS, 1>(a, s);
     }
     return direct(1, q4_kernel<XT, G, MINS, 1>);

@@ -19,13 +19,25 @@ struct DeviceScope {
     }
 };
 
-#define OPS_REFUSE(...) do { c->err = fmt(__VA_ARGS__); return HIPVOC_E_ARG; } while (0)
+// Calls on one handle may come from several threads: what they share is the text of the last failure and the deferred error word.
+static std::mutex g_ops_sync;
+static int ops_fail(Ctx *c, int code, const std::string &why) {
+    std::lock_guard<std::mutex> lock(g_ops_text);
+    c->err = why;
+    return code;
+}
+
 #define OPS(h)                                                                                                             \
     Ctx *c = (Ctx *)(h);                                                                                                   \
     if (!c) return HIPVOC_E_ARG;                                                                                           \
-    if (!c->is_ops) { c->err = "this handle is no operator handle (hipvoc_ops_open)"; return HIPVOC_E_ARG; }               \
+    if (!c->is_ops) return ops_fail(c, HIPVOC_E_ARG, "this handle is no operator handle (hipvoc_ops_open)");               \
     DeviceScope scope(c->device);                                                                                          \
-    if (!scope.ok) { c->err = "hipSetDevice failed"; return HIPVOC_E_HIP; }
+    if (!scope.ok) return ops_fail(c, HIPVOC_E_HIP, "hipSetDevice failed");
+#define OPS_HIP(expr)                                                                                                      \
+    do {                                                                                                                   \
+        const hipError_t e__ = (expr);                                                                                     \
+        if (e__ != hipSuccess) return ops_fail(c, HIPVOC_E_HIP, fmt("%s failed: %s", #expr, hipGetErrorString(e__)));      \
+    } while (0)
 
 // a stream of another device would run the kernels there
 static int ops_stream(Ctx *c, void *stream) {
@@ -33,22 +45,20 @@ static int ops_stream(Ctx *c, void *stream) {
     hipDevice_t dev = c->device;
     if (hipStreamGetDevice((hipStream_t)stream, &dev) != hipSuccess) {
         (void)hipGetLastError();
-        OPS_REFUSE("no such stream");
+        return ops_fail(c, HIPVOC_E_ARG, "no such stream");
     }
-    if (dev != c->device) OPS_REFUSE("the stream is of device %d, the handle of device %d", (int)dev, c->device);
+    if (dev != c->device) return ops_fail(c, HIPVOC_E_ARG, fmt("the stream is of device %d, the handle of device %d", (int)dev, c->device));
     return HIPVOC_OK;
 }
 
 static int ops_launched(Ctx *c, const char *what, hipError_t e) {
-    if (e == hipSuccess) return HIPVOC_OK;
-    c->err = fmt("%s: launch failed: %s", what, hipGetErrorString(e));
-    return HIPVOC_E_HIP;
+    return e == hipSuccess ? HIPVOC_OK : ops_fail(c, HIPVOC_E_HIP, fmt("%s: launch failed: %s", what, hipGetErrorString(e)));
 }
 
 static int ops_move(Ctx *c, const char *what, bool write, const hipvoc_kv_cache *cache, void *k, void *v, int64_t ks, int64_t vs, int dtype,
                     const hipvoc_kv_rows *rows, int n_rows, void *stream) {
-    c->err = check_move(cache, k, v, ks, vs, dtype, rows, n_rows);
-    if (!c->err.empty()) return HIPVOC_E_ARG;
+    const std::string why = check_move(cache, k, v, ks, vs, dtype, rows, n_rows);
+    if (!why.empty()) return ops_fail(c, HIPVOC_E_ARG, why);
     const int rc = ops_stream(c, stream);
     if (rc || n_rows == 0 || rows->n_seqs == 0) return rc;
     const KvMoveArgs a = {*cache, *rows, __builtin_ctz((unsigned)cache->page), k, v, ks, vs, dtype, n_rows, c->d_err};
@@ -59,21 +69,24 @@ static int ops_move(Ctx *c, const char *what, bool write, const hipvoc_kv_cache 
 static int ops_collect(Ctx *c, hipStream_t stream) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (stream && hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
-        OPS_REFUSE("the stream is being captured: it cannot be waited for");
+        return ops_fail(c, HIPVOC_E_ARG, "the stream is being captured: it cannot be waited for");
     int bits = 0;
-    HIPCHK(launch_take_error(c->d_err, stream));
-    HIPCHK(hipStreamSynchronize(stream));
-    HIPCHK(hipMemcpyWithStream(&bits, c->d_err + 1, sizeof bits, hipMemcpyDeviceToHost, stream));
+    {
+        std::lock_guard<std::mutex> lock(g_ops_sync);      // d_err[1] is one caller's at a time
+        OPS_HIP(launch_take_error(c->d_err, stream));
+        OPS_HIP(hipStreamSynchronize(stream));
+        OPS_HIP(hipMemcpyWithStream(&bits, c->d_err + 1, sizeof bits, hipMemcpyDeviceToHost, stream));
+    }
     if (!bits) return HIPVOC_OK;
-    c->err = fmt("on the device:%s%s%s", bits & OPS_ERR_POSITION ? " a row's position outside its sequence's pages;" : "",
-                 bits & OPS_ERR_PAGE ? " a page number outside the cache;" : "", bits & OPS_ERR_LENGTH ? " a length outside 0 .. max_len;" : "");
-    return HIPVOC_E_CODE;
+    return ops_fail(c, HIPVOC_E_CODE, fmt("on the device:%s%s%s", bits & OPS_ERR_POSITION ? " a row's position outside its sequence's pages;" : "",
+                                          bits & OPS_ERR_PAGE ? " a page number outside the cache;" : "",
+                                          bits & OPS_ERR_LENGTH ? " a length outside 0 .. max_len;" : ""));
 }
 
 static int ops_sync_device(Ctx *c) {
     DeviceScope scope(c->device);
-    if (!scope.ok) { c->err = "hipSetDevice failed"; return HIPVOC_E_HIP; }
-    HIPCHK(hipDeviceSynchronize());
+    if (!scope.ok) return ops_fail(c, HIPVOC_E_HIP, "hipSetDevice failed");
+    OPS_HIP(hipDeviceSynchronize());
     return ops_collect(c, nullptr);
 }
 
@@ -141,7 +154,7 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
 }
 
 size_t hipvoc_attention_workspace(const hipvoc_kv_cache *cache, int n_heads, int n_seqs, int max_len, int window) {
-    if (!cache || cache->kv_heads < 1 || n_heads < 1 || n_seqs < 1 || max_len < 1 || window < 0) return 0;
+    if (!cache || cache->kv_heads < 1 || n_heads < 1 || n_heads % cache->kv_heads || n_seqs < 1 || max_len < 1 || window < 0) return 0;
     // the act type is not asked for: what either kernel needs
     const bool coded = cache->dtype == HIPVOC_T_INT8 || cache->dtype == HIPVOC_T_E4M3;
     return std::max(attention_plan(HIPVOC_T_F32, coded, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window).bytes,
@@ -153,9 +166,9 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
                      int window, float scale, void *workspace, size_t workspace_bytes, void *stream) {
     return guarded(h, [&]() -> int {
         OPS(h);
-        c->err = check_attention(cache, q, q_stride, out, out_stride, lse, dtype, n_heads, table, table_stride, table_width, lens, n_seqs, max_len, window,
-                                 scale, workspace, workspace_bytes);
-        if (!c->err.empty()) return HIPVOC_E_ARG;
+        const std::string why = check_attention(cache, q, q_stride, out, out_stride, lse, dtype, n_heads, table, table_stride, table_width, lens,
+                                                n_seqs, max_len, window, scale, workspace, workspace_bytes);
+        if (!why.empty()) return ops_fail(c, HIPVOC_E_ARG, why);
         const int rc = ops_stream(c, stream);
         if (rc || n_seqs == 0) return rc;
         const AttnPlan p = attention_plan(dtype, cache->dtype != dtype, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
@@ -193,8 +206,8 @@ int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *res
                        int cols, void *stream) {
     return guarded(h, [&]() -> int {
         OPS(h);
-        c->err = check_norm(x, x_stride, residual, residual_stride, weight, sum, sum_stride, y, y_stride, scales, dtype, out_dtype, group, eps, rows, cols);
-        if (!c->err.empty()) return HIPVOC_E_ARG;
+        const std::string why = check_norm(x, x_stride, residual, residual_stride, weight, sum, sum_stride, y, y_stride, scales, dtype, out_dtype, group, eps, rows, cols);
+        if (!why.empty()) return ops_fail(c, HIPVOC_E_ARG, why);
         const int rc = ops_stream(c, stream);
         if (rc || rows == 0) return rc;
         NormArgs a = {x, residual, weight, sum, y, scales, x_stride, residual ? residual_stride : 0, sum_stride, y_stride, dtype, out_dtype, group, eps, rows, cols};
@@ -207,8 +220,8 @@ int hipvoc_q4_matvec(void *h, const uint8_t *codes, const void *scales, const vo
                      void *stream) {
     return guarded(h, [&]() -> int {
         OPS(h);
-        c->err = check_q4(codes, scales, mins, n_out, n_in, group, x, x_stride, x_dtype, x_scale, x_groups, y, y_stride, y_dtype, n_rows);
-        if (!c->err.empty()) return HIPVOC_E_ARG;
+        const std::string why = check_q4(codes, scales, mins, n_out, n_in, group, x, x_stride, x_dtype, x_scale, x_groups, y, y_stride, y_dtype, n_rows);
+        if (!why.empty()) return ops_fail(c, HIPVOC_E_ARG, why);
         const int rc = ops_stream(c, stream);
         if (rc || n_rows == 0 || n_out == 0) return rc;
         Q4Args a = {codes, scales, mins, n_out, n_in, group, x, x_stride, x_dtype, x_scale, x_groups, y, y_stride, y_dtype, n_rows};

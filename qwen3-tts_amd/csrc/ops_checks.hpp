@@ -61,6 +61,7 @@ static inline std::string check_move(const hipvoc_kv_cache *cache, const void *k
     if (!why.empty()) return why;
     if (n_rows < 0 || n_rows > 1 << 28) return ops_say("n_rows %d is not in 0 .. 2^28", n_rows);
     if (n_rows == 0 || r->n_seqs == 0) return "";
+    if ((int64_t)n_rows * kv_parts(cache->kv_heads, cache->head_dim) * 64 + 256 > OPS_MAX_THREADS) return "n_rows: too many for one call with that many heads";
     if (!k || !v || !r->cu || !r->first) return "null pointer";
     if (((uintptr_t)r->cu | (uintptr_t)r->first) & 3) return "cu / first are not aligned to their type";
     const int64_t row = (int64_t)cache->kv_heads * cache->head_dim;
@@ -79,7 +80,7 @@ static inline std::string check_attention(const hipvoc_kv_cache *cache, const vo
     if (n_heads < 1 || n_heads % cache->kv_heads || n_heads > 16384) return ops_say("n_heads %d is no multiple of kv_heads %d (up to 16384)", n_heads, cache->kv_heads);
     if (max_len < 0 || max_len > (int64_t)table_width * cache->page) return ops_say("max_len %d does not fit %d pages of %d", max_len, table_width, cache->page);
     if (window < 0) return "window must not be negative";
-    if (!(scale - scale == 0.f)) return "scale must be finite";
+    if (!(scale > -1e38f && scale < 1e38f)) return "scale must be finite";
     if (n_seqs == 0) return "";
     if (!q || !out || !lens) return "null pointer";
     if (((uintptr_t)lens | (uintptr_t)lse) & 3) return "lens / lse are not aligned to their type";
@@ -87,6 +88,7 @@ static inline std::string check_attention(const hipvoc_kv_cache *cache, const vo
     if (q_stride < row || out_stride < row || q_stride > OPS_MAX_STRIDE || out_stride > OPS_MAX_STRIDE) return "q_stride / out_stride shorter than n_heads * head_dim";
     if (odd16(q) || odd16(out) || odd16(q_stride, dtype) || odd16(out_stride, dtype)) return "rows must be 16-byte aligned";
     const AttnPlan p = attention_plan(dtype, cache->dtype != dtype, cache->head_dim, cache->kv_heads, n_heads, n_seqs, max_len, window);
+    if (!p.workers && (int64_t)n_seqs * p.heads * 256 > OPS_MAX_THREADS) return "n_seqs: too many for one call with that many heads";
     if (p.bytes && (!workspace || odd16(workspace) || workspace_bytes < p.bytes))
         return ops_say("workspace: %zu bytes needed, 16-byte aligned (hipvoc_attention_workspace)", p.bytes);
     return "";
@@ -98,7 +100,7 @@ static inline std::string check_norm(const void *x, int64_t x_stride, const void
     const bool coded = out_dtype == HIPVOC_T_INT8 || out_dtype == HIPVOC_T_E4M3;
     if (!act_type(dtype)) return "dtype must be F32, F16 or BF16";
     if (!coded && out_dtype != dtype) return "out_dtype must be dtype, INT8 or E4M3";
-    if (rows < 0 || cols < 1 || cols > 1 << 20) return ops_say("rows %d, cols %d (1 .. 2^20)", rows, cols);
+    if (rows < 0 || rows >= 1 << 22 || cols < 1 || cols > 1 << 20) return ops_say("rows %d (under 2^22), cols %d (1 .. 2^20)", rows, cols);
     if (coded ? group != 0 && ((group != 32 && group != 64 && group != 128) || cols % group) : group != 0)
         return ops_say("group %d must be 0, or for 8-bit rows 32, 64 or 128 and a divisor of cols %d", group, cols);
     if (!(eps >= 0.f && eps < 1e30f)) return "eps must be finite and not negative";

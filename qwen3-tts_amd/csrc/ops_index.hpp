@@ -45,6 +45,12 @@ OPS_FN int64_t row_position(int t, int cu, int first, int table_width, int page_
 }
 OPS_FN bool page_ok(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages; }
 
+// A launch's threads have to be counted in 32 bits.
+static const int64_t OPS_MAX_THREADS = ((int64_t)1 << 32) - 1;
+// Waves that have a token's 2 * kv_heads rows: a wave has KV_U times as many as its lanes hold at eight values each
+enum { KV_U = 4 };
+OPS_FN int kv_parts(int kv_heads, int head_dim) { return (2 * kv_heads * head_dim + 512 * KV_U - 1) / (512 * KV_U); }
+
 struct AttnPlan { int heads, workers, least; size_t bytes; };
 enum { ATTN_MAX_SEQS = 1024, ATTN_WHOLE_TILES = 24 };      // sequences whose lengths a workgroup adds up; tiles that are not worth a cut
 // How a call is cut, from sizes alone.  `heads`: (key head, tile of query heads) pairs of a sequence; a workgroup each (workers 0) if the spans

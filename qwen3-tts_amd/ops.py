@@ -183,6 +183,8 @@ class HipOps:
         if t.device != self.device:
             self._elsewhere(name, t)
         rows = shape[0]
+        if rows >> 31:
+            _refuse(f"{name} has {rows} rows")
         return rows, stride[0] if rows > 1 else heads * hd
 
     def _matrix(self, name, t):
@@ -196,6 +198,8 @@ class HipOps:
             _refuse(f"{name} must have contiguous rows")
         if t.device != self.device:
             self._elsewhere(name, t)
+        if rows >> 31 or cols >> 31:
+            _refuse(f"{name} is {rows} by {cols}")
         return rows, cols, stride[0] if rows > 1 else cols
 
     # ---- the paged cache -----------------------------------------------------------------
@@ -251,6 +255,8 @@ class HipOps:
         softmax's sum [seqs, heads] float32.  max_len: a bound on lens the host knows (default: all the table's pages hold)."""
         if cache.device != self.device:
             self._elsewhere("the cache", cache)
+        if q.dim() != 3:
+            _refuse("q must be [seqs, heads, head_dim]")
         hd, heads = cache.head_dim, q.shape[1]
         n, qs = self._heads("q", q, heads, hd)
         tp, stride, width, nt = self._table(table)
@@ -321,6 +327,8 @@ class HipOps:
         if len(cs) != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
             _refuse("codes must be a contiguous uint8 [n_out, n_in / 2]")
         n_out, n_in = cs[0], cs[1] * 2
+        if n_out >> 31 or n_in >> 31:
+            _refuse(f"codes are {n_out} rows of {n_in}")
         if len(ss) != 2 or ss[0] != n_out or scales.dtype != torch.float16 or not scales.is_contiguous() or ss[1] < 1 or n_in % ss[1]:
             _refuse("scales must be a contiguous float16 [n_out, n_in / group]")
         here, mp, xp = self.device, None, None

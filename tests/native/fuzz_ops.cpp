@@ -144,6 +144,17 @@ static void moves() {
     b.table_width = 1 << 28; b.table_stride = 1 << 28; REFUSED(check_move(&c, k, v, 128, 128, 2, &b, 5)); b = r;
     b.n_seqs = 70000; REFUSED(check_move(&c, k, v, 128, 128, 2, &b, 5)); b = r;
     b.n_seqs = -1; REFUSED(check_move(&c, k, v, 128, 128, 2, &b, 5));
+    // a launch's threads count in 32 bits
+    for (int hd = 64; hd <= 128; hd *= 2)
+        for (int heads = 1; heads <= 1024; heads += heads < 40 ? 1 : 123) {
+            c.head_dim = hd; c.kv_heads = heads; c.page_stride = (int64_t)heads * 16 * hd;
+            const int64_t parts = kv_parts(heads, hd), row = (int64_t)heads * hd;
+            CHECK(parts * KV_U * 64 * 8 >= 2 * row && (parts - 1) * KV_U * 64 * 8 < 2 * row);
+            const int most = (int)std::min<int64_t>(1 << 28, ((int64_t)1 << 32) / 64 / parts - 8);
+            FINE(check_move(&c, k, v, row, row, 2, &r, most));
+            CHECK((most * parts + 3) / 4 * 256 < (int64_t)1 << 32);
+            if (most < 1 << 28) REFUSED(check_move(&c, k, v, row, row, 2, &r, most + 16));
+        }
 }
 
 struct A {
@@ -169,6 +180,7 @@ static void attentions() {
     a.window = -1; REFUSED(a.go()); a = A();
     a.scale = 1e30f * 1e30f; REFUSED(a.go()); a = A();
     a.scale = a.scale * 0.f / 0.f; REFUSED(a.go()); a = A();
+    a.scale = 3e38f; REFUSED(a.go()); a = A();
     a.q = nullptr; REFUSED(a.go()); a = A();
     a.out = (void *)0x2001; REFUSED(a.go()); a = A();
     a.lens = nullptr; REFUSED(a.go()); a = A();
@@ -179,6 +191,8 @@ static void attentions() {
     a.bytes = 16; REFUSED(a.go()); a = A();
     a.ts = 63; REFUSED(a.go()); a = A();
     a.seqs = 0; a.q = nullptr; FINE(a.go()); a = A();
+    a.seqs = 65535; FINE(a.go());
+    a.c.kv_heads = 512; a.c.page_stride = 512 * 16 * 64; a.heads = 512; a.qs = a.os = 512 * 64; REFUSED(a.go()); a = A();
     a.max_len = 0; a.ws = nullptr; a.bytes = 0; FINE(a.go());
 }
 
@@ -204,6 +218,8 @@ static void norms() {
     REFUSED(go(2, 2, 0, 3, 0, 96, 1e-6f, 0x100, 0, 0, 0));
     REFUSED(go(2, 2, 0, 3, (1 << 20) + 1, 1 << 21, 1e-6f, 0x100, 0, 0, 0));
     REFUSED(go(2, 2, 0, -1, 96, 96, 1e-6f, 0x100, 0, 0, 0));
+    FINE(go(2, 2, 0, (1 << 22) - 1, 96, 96, 1e-6f, 0x100, 0, 0, 0));
+    REFUSED(go(2, 2, 0, 1 << 22, 96, 96, 1e-6f, 0x100, 0, 0, 0));
     REFUSED(go(2, 2, 0, 3, 96, 96, 1e-6f, 0x101, 0, 0, 0));
     REFUSED(go(0, 0, 0, 3, 96, 96, 1e-6f, 0x102, 0, 0, 0));
     REFUSED(go(2, 2, 0, 3, 96, 96, 1e-6f, 0, 0, 0, 0));

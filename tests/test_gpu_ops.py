@@ -103,8 +103,8 @@ def attention_ref(P, q, scale, window):
     b, heads, hd = q.shape
     outs, lses, bo, bl = [], [], [], []
     rep = heads // P.kv
-    # the weights' rounding for the product with V: one f16, or two bf16, the second holding what the first leaves over
-    p16 = 0.0 if P.act == torch.float32 else u(torch.float16) if P.act == torch.float16 and P.store == "same" else u(torch.bfloat16) ** 2
+    # the weights' rounding for the product with V: two f16 or two bf16, the second holding what the first leaves over
+    p16 = 0.0 if P.act == torch.float32 else u(torch.float16 if P.act == torch.float16 and P.store == "same" else torch.bfloat16) ** 2
     for s in range(b):
         n = P.lens[s]
         lo = max(0, n - window) if window else 0
@@ -125,8 +125,8 @@ def attention_ref(P, q, scale, window):
         m = n - lo
         err = wv * (2 * delta[:, None] + p16 + (2 * m + 16) * U32)
         if P.act == torch.float16 and P.store == "same":
-            # weights below the type's normal range (of the largest weight, 1 before normalisation) are off by half its smallest step
-            err = err + w.amax(-1)[:, None] * m * 2.0 ** -25 * v.abs().amax(1)
+            # weights below the type's normal range (the largest weight being 2^15 there) are off by half its smallest step
+            err = err + w.amax(-1)[:, None] * m * 2.0 ** -40 * v.abs().amax(1)
         outs.append(out)
         bo.append(err + u(P.act) * (out.abs() + err) + 2.0 ** -24 * (P.act == torch.float16))
         lse = torch.logsumexp(score, -1)
@@ -154,7 +154,7 @@ def check_attention(ops, P, q, scale=None, window=0, max_len=None, **kw):
 # the cache
 @pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("store", ["same", "int8", "e4m3"])
-@pytest.mark.parametrize("kv,hd,page", [(1, 64, 8), (3, 128, 16), (8, 64, 256)])
+@pytest.mark.parametrize("kv,hd,page", [(1, 64, 8), (3, 128, 16), (8, 64, 256), (20, 128, 8), (33, 64, 8)])
 def test_kv_write_and_read(ops, act, store, kv, hd, page):
     """Codes and scales bit for bit, the values read back bit for bit, unwritten places and padding rows untouched."""
     P = Paged(ops, [0, 5, page + 3, 1], kv, hd, page, act, store, seed=3, width=4)
@@ -314,6 +314,59 @@ def test_attention_split_and_joined(ops, act, store, hd, rep):
     assert torch.equal(a[0], again[0]) and torch.equal(a[1], again[1])         # the order of every sum is fixed
     assert b[0].shape == a[0].shape
     check_attention(ops, P, q, max_len=5003, window=3000)
+
+
+# bounds over 768 keys: the tiles of all sequences are shared out over the card
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("store", ["same", "int8", "e4m3"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv,rep,page", [(1, 1, 8), (2, 2, 16), (3, 4, 256), (1, 17, 64), (2, 8, 32)])
+def test_attention_shared_out(ops, act, store, hd, kv, rep, page):
+    """Empty and short sequences among long ones, so that a wave's share has many pieces; windows that are short, long and over the bound."""
+    P = Paged(ops, [0, 1, 33, 800, 0, 0, 5, 64, 1500, 31, 300, 0], kv, hd, page, act, store, seed=kv * 10 + rep, together=page == 16)
+    q = rnd((12, kv * rep, hd), ACT[act], 5)
+    check_attention(ops, P, q)
+    check_attention(ops, P, q, window=781)
+    check_attention(ops, P, q, window=4000)
+
+
+@pytest.mark.parametrize("act,store", [("f32", "same"), ("bf16", "int8"), ("f16", "same")])
+@pytest.mark.parametrize("n", [1023, 1024, 1025])
+def test_attention_many_sequences(ops, act, store, n):
+    """As many sequences as a workgroup adds up, and one more: those are not cut."""
+    lens = [(i * 37) % 90 for i in range(n)]
+    lens[n // 2], lens[-1] = 900, 77
+    P = Paged(ops, lens, 1, 64, 16, act, store, seed=n)
+    check_attention(ops, P, rnd((n, 2, 64), ACT[act], 3))
+
+
+def test_attention_all_empty(ops):
+    for lens, bound in (([0, 0, 0], None), ([0], 0), ([0, 0], 5000)):
+        P = Paged(ops, lens, 2, 64, 8, "bf16", seed=1, width=700)
+        out, lse = ops.attention(torch.full((len(lens), 4, 64), 3.0, dtype=torch.bfloat16, device="cuda"), P.cache, P.table, P.lens_dev, max_len=bound, lse=True)
+        ops.sync()
+        assert not bool(out.any()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16", "f32"])
+def test_attention_many_small_weights(ops, act):
+    """One key far above 40000 others, each of which has e^-16.25 of its weight, 1.47 * 2^-24: together they are the result."""
+    n, page, less = 40001, 64, 16.25
+    pages = -(-n // page)
+    k = torch.zeros((pages, 1, page, 64), dtype=ACT[act], device="cuda")
+    v = torch.ones_like(k)
+    k[..., 0] = -less
+    k[0, 0, 0], v[0, 0, 0] = 0, 0
+    q = torch.zeros((1, 1, 64), dtype=ACT[act], device="cuda")
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out = ops.attention(q, ops.kv_cache(k, v), table, ints([n]), scale=1.0, max_len=n)
+    ops.sync()
+    p = (n - 1) * math.exp(-less)
+    ref = p / (1 + p)
+    delta = (64 + 8) * U32 * less + 8 * U32 * (1 + less) + 2.0 ** -21                  # as in attention_ref
+    rel = 2 * delta + (2 * n + 16) * U32 + u(ACT[act]) + u(torch.bfloat16) ** 2
+    assert float((out.cpu().double() - ref).abs().max()) <= rel * ref
 
 
 def test_attention_lse_joins_two_caches(ops):
@@ -584,6 +637,63 @@ def test_q4_matvec_larger(ops, act, m, n, k):
     check_q4(ops, n, k, 32, False, rnd((m, k), ACT[act], 2), seed=4)
 
 
+# the kernels for many weight rows: from 16384 and 65536 of them (32-bit rows: 8192 and 32768)
+@pytest.mark.parametrize("act,n,group,mult,mins,m", [
+    ("bf16", 16384, 64, 5, True, 3), ("f16", 16390, 32, 33, False, 17), ("bf16", 65541, 128, 3, True, 1), ("f16", 65536, 64, 18, False, 16),
+    ("bf16", 65537, 32, 40, True, 2), ("bf16", 16385, 32, 131, True, 5), ("f16", 65540, 32, 128, True, 2), ("bf16", 65536, 32, 123, False, 1),
+    ("f16", 65536, 32, 125, False, 33), ("bf16", 16384, 32, 1, True, 1), ("f32", 8192, 64, 9, True, 2), ("f32", 8199, 32, 130, False, 1),
+    ("f32", 32769, 64, 5, False, 17), ("f32", 32768, 32, 33, True, 3), ("f32", 32780, 32, 140, True, 1), ("int8", 16399, 64, 5, False, 3),
+    ("int8", 16384, 32, 132, True, 18), ("int8", 65536, 32, 127, True, 2), ("int8", 65551, 128, 9, False, 1), ("int8", 100, 32, 300, True, 4),
+    ("bf16", 100, 32, 300, True, 4), ("f32", 70, 32, 257, False, 17)])
+def test_q4_matvec_many_weight_rows(ops, act, n, group, mult, mins, m):
+    """Checked against 64 bits for rows at both ends and a thousand in between; K in whole slabs of 128 columns and not, over 128 groups."""
+    k = group * mult
+    g = torch.Generator().manual_seed(n + mult)
+    scale = None
+    if act == "int8":
+        x = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8)
+        scale = torch.rand((m, mult if mult % 2 else 1), generator=g) * 0.02
+    else:
+        x = rnd((m, k), ACT[act], m + n, 2.0)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scales = (torch.rand((n, mult), generator=g) * 0.1 - 0.03).to(torch.float16)
+    least = (torch.randn((n, mult), generator=g) * 0.3).to(torch.float16) if mins else None
+    y = ops.q4_matvec(codes.cuda(), scales.cuda(), x.cuda(), mins=None if least is None else least.cuda(), x_scale=None if scale is None else scale.cuda())
+    ops.sync()
+    pick = torch.unique(torch.cat([torch.arange(min(n, 80)), torch.arange(max(0, n - 300), n), torch.randint(0, n, (1000,), generator=g)]))
+    c = torch.stack((codes[pick] & 15, codes[pick] >> 4), -1).reshape(len(pick), k).double()
+    s = scales[pick].double().repeat_interleave(group, 1)
+    low = least[pick].double().repeat_interleave(group, 1) if mins else 0 * s
+    w = s * c + low if mins else s * (c - 8)
+    xv = x.double()
+    if scale is not None:
+        xv = xv * (scale.double().repeat_interleave(group, 1) if scale.shape[1] > 1 else scale.double())
+    ref = xv @ w.t()
+    mag = xv.abs() @ (55 * s.abs() + low.abs()).t()                                       # as in check_q4
+    bound = mag * ((k + 16) * U32) + u(y.dtype) * ref.abs() + 2.0 ** -25 * (y.dtype == torch.float16)
+    d = (y.cpu()[:, pick].double() - ref).abs()
+    assert y.shape == (m, n) and bool((d <= bound * (1 + u(y.dtype))).all()), float((d / bound).max())
+
+
+def test_q4_matvec_wide_captured_first(ops):
+    """The kernel that asks for more than the default of shared memory, first called under capture."""
+    n, k = 65536, 256
+    codes, scales, _, _, _ = q4_weights(n, k, 128, False, 1)
+    codes, scales = codes.cuda(), scales.cuda()
+    x = torch.zeros((2, k), dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.q4_matvec(codes, scales, x)
+    for rep in range(3):
+        x.copy_(rnd((2, k), torch.float16, rep))
+        want = ops.q4_matvec(codes, scales, x)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and bool(y.any())
+
+
 def test_q4_matvec_strides_extremes_and_repeat(ops):
     """Rows inside a wider tensor; codes 0 and 15 throughout; large and small activations; the same bits every time."""
     wide = rnd((5, 512), torch.bfloat16, 5).cuda()
@@ -841,3 +951,49 @@ def test_refusals(pkg, ops):
         assert e.value.code == -1, (i, str(e.value))
     P.lens_dev = ints([9, 12])
     check_attention(ops, P, q)
+
+
+def test_refusals_of_shapes(pkg, ops):
+    """What the C side cannot see in a tensor, or would have to divide by."""
+    P = Paged(ops, [9], 8, 64, 8, "bf16")
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    for bad in [lambda: ops.attention(bf(1, 4, 64), P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 12, 64), P.cache, P.table, P.lens_dev),
+                lambda: ops.attention(bf(64), P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 0, 64), P.cache, P.table, P.lens_dev),
+                lambda: ops.add_rmsnorm(bf(1, 8).expand(1 << 22, 8).contiguous(), bf(8)), lambda: ops.add_rmsnorm(bf(1, 8).expand(4, 8), bf(8))]:
+        with pytest.raises(pkg.HipVocError) as e:
+            bad()
+        assert e.value.code == -1 and len(str(e.value)) > 5
+    ops.sync()
+
+
+def test_calls_from_several_threads(pkg, ops):
+    """One handle, four threads with a stream each: sound calls give what they give alone, refused ones their code and a text."""
+    import threading
+    w = (1 + 0.1 * rnd((512,), torch.float32, 1)).cuda()
+    xs = [rnd((33, 512), torch.float32, 10 + i).cuda() for i in range(4)]
+    want = [ops.add_rmsnorm(x, w)[1].clone() for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    got = ops.add_rmsnorm(xs[i], w)[1]
+                    try:
+                        ops.add_rmsnorm(xs[i], w, eps=-1.0)
+                        wrong.append("not refused")
+                    except pkg.HipVocError as e:
+                        if e.code != -1 or "eps" not in str(e):
+                            wrong.append(str(e))
+                    ops.sync()
+                    if not torch.equal(got, want[i]):
+                        wrong.append("differs")
+        except Exception as e:  # noqa: BLE001
+            wrong.append(repr(e))
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]

@@ -54,6 +54,21 @@ def test_no_cpu_fallback_for_the_operators(pkg):
     assert lib.hipvoc_attention_workspace(None, 4, 4, 100, 0) == 0
 
 
+def test_workspace_of_any_sizes(pkg):
+    """A size function answers whatever it is asked: heads that do not divide, nothing to do, extreme lengths."""
+    import torch
+    lib = pkg.ops._lib()
+    k = torch.zeros((2, 8, 16, 64), dtype=torch.bfloat16)
+    c = pkg.KvCache(k, k.clone())
+    for heads in (0, -8, 4, 12, 1):                                     # fewer than, or no multiple of, the eight key heads
+        assert lib.hipvoc_attention_workspace(c._p, heads, 4, 5000, 0) == 0
+    assert lib.hipvoc_attention_workspace(c._p, 16, 4, 768, 0) == 0 and lib.hipvoc_attention_workspace(c._p, 16, 4, 5000, 700) == 0
+    assert 0 < lib.hipvoc_attention_workspace(c._p, 16, 4, 5000, 0) < 1 << 24
+    assert lib.hipvoc_attention_workspace(c._p, 16, 0, 5000, 0) == 0 and lib.hipvoc_attention_workspace(c._p, 16, 4, 0, 0) == 0
+    assert lib.hipvoc_attention_workspace(c._p, 16, 2000, 5000, 0) == 0
+    assert lib.hipvoc_attention_workspace(c._p, 16384, 1024, 2 ** 31 - 1, 0) > 1 << 32
+
+
 def test_what_is_refused_and_where_the_kernels_read(tmp_path):
     """tests/native/fuzz_ops.cpp under the host sanitizers: chunks of a sequence cover what its token sees and nothing else, for sound,
     extreme and malformed lengths; positions and pages out of range are never followed; every refusal of the C entry points."""
