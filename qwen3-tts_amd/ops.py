@@ -1,11 +1,12 @@
-"""ctypes binding of the token-step operators of libhipvoc.so (include/hipvoc_ops.h).
+"""The token-step operators of libhipvoc.so (include/hipvoc_ops.h) on torch tensors.
 
 ``HipOps.open(device)`` gives a handle; its methods take torch tensors of that device and enqueue on torch's current stream
 of it, so they can be captured into a graph with the rest of a step.  They allocate their results (and a workspace, where one
 is needed) as torch operations do; the C entry points take the caller's memory.  A refused call raises HipVocError before
 anything is launched; what only the device can see (a page number, a length) is raised by ``sync()``.
 
-There is NO fallback: if the shared library is missing or no HIP device is present, opening raises.
+The tensors are looked at in _ops_torch.so (csrc/ops_torch.cpp), which calls the C entry points; here they have their names.
+There is NO fallback: if a shared library is missing or no HIP device is present, opening raises.
 """
 from __future__ import annotations
 
@@ -55,6 +56,7 @@ def _lib():
 
 
 torch = None
+_native = None                  # _ops_torch.so
 _types = {}                     # torch dtype -> HIPVOC_T_*
 
 
@@ -104,11 +106,21 @@ class KvCache:
         self._p = C.addressof(self._c)
 
 
+def _bind_native():
+    global _native
+    if _native is None:
+        _bind_torch()
+        from . import _ops_torch as module
+        L = _lib()
+        at = lambda name: C.cast(getattr(L, name), C.c_void_p).value  # noqa: E731
+        module.bind(HipVocError, *[at("hipvoc_" + n) for n in ("kv_write", "kv_read", "attention_workspace", "attention", "add_rmsnorm", "q4_matvec", "last_error")])
+        _native = module
+
+
 class HipOps:
     """The operators of one token step on one MI355X."""
 
     def __init__(self, handle, lib, device: int):
-        _bind_torch()
         self._h = handle
         self._L = lib
         self.device = torch.device("cuda", device)
@@ -120,6 +132,11 @@ class HipOps:
         h = L.hipvoc_ops_open(device)
         if not h:
             raise HipVocError(-6, L.hipvoc_last_error(None).decode())
+        try:
+            _bind_native()
+        except BaseException:
+            L.hipvoc_free(h)
+            raise
         return cls(h, L, device)
 
     def close(self):
@@ -133,9 +150,6 @@ class HipOps:
         except Exception:
             pass
 
-    def _failed(self, rc: int):
-        raise HipVocError(rc, self._L.hipvoc_last_error(self._h).decode() if self._h else "the handle is closed")
-
     @property
     def stream(self) -> int:
         """torch's current stream of the handle's device, where the calls are enqueued."""
@@ -145,219 +159,40 @@ class HipOps:
         """Waits for the current stream and raises what the device found wrong since the last time."""
         rc = self._L.hipvoc_ops_sync(self._h, self.stream)
         if rc:
-            self._failed(rc)
-
-    # ---- what a call looks at in its tensors (a step makes these calls per layer: each attribute is asked for once) -----
-    def _elsewhere(self, name, t):
-        _refuse(f"{name} is on {t.device}, the handle on {self.device}")
-
-    def _here(self, name, t):
-        if t is not None and t.device != self.device:
-            self._elsewhere(name, t)
-
-    def _ints(self, name, t, n):
-        """Address of a contiguous int32 vector of n values."""
-        if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-            _refuse(f"{name} must be a contiguous int32 vector of {n}")
-        if t.device != self.device:
-            self._elsewhere(name, t)
-        return t.data_ptr()
-
-    def _table(self, t):
-        """(address, stride, width, rows) of a page table."""
-        shape = t.shape
-        if t.dtype != torch.int32 or len(shape) != 2:
-            _refuse("table must be int32 [seqs, pages]")
-        stride = t.stride()
-        if shape[1] > 1 and stride[1] != 1:
-            _refuse("table must have contiguous rows")
-        if t.device != self.device:
-            self._elsewhere("table", t)
-        return t.data_ptr(), stride[0], shape[1], shape[0]
-
-    def _heads(self, name, t, heads, hd):
-        """(rows, row stride) of [rows, heads, head_dim] with contiguous rows."""
-        shape, stride = t.shape, t.stride()
-        if len(shape) != 3 or shape[1] != heads or shape[2] != hd or stride[2] != 1 or (heads > 1 and stride[1] != hd):
-            _refuse(f"{name} must be [rows, {heads}, {hd}] with contiguous rows")
-        if t.device != self.device:
-            self._elsewhere(name, t)
-        rows = shape[0]
-        if rows >> 31:
-            _refuse(f"{name} has {rows} rows")
-        return rows, stride[0] if rows > 1 else heads * hd
-
-    def _matrix(self, name, t):
-        """(rows, columns, row stride) of a matrix with contiguous rows."""
-        shape = t.shape
-        if len(shape) != 2:
-            _refuse(f"{name} must be a matrix")
-        rows, cols = shape
-        stride = t.stride()
-        if stride[1] != 1 and cols > 1:
-            _refuse(f"{name} must have contiguous rows")
-        if t.device != self.device:
-            self._elsewhere(name, t)
-        if rows >> 31 or cols >> 31:
-            _refuse(f"{name} is {rows} by {cols}")
-        return rows, cols, stride[0] if rows > 1 else cols
+            raise HipVocError(rc, self._L.hipvoc_last_error(self._h).decode() if self._h else "the handle is closed")
 
     # ---- the paged cache -----------------------------------------------------------------
     def kv_cache(self, k, v, k_scale=None, v_scale=None) -> KvCache:
-        self._here("k", k)
+        if k.device != self.device:
+            _refuse(f"k is on {k.device}, the handle on {self.device}")
         return KvCache(k, v, k_scale, v_scale)
-
-    def _rows(self, table, cu, first):
-        tp, stride, width, n = self._table(table)
-        return _Rows(tp, self._ints("cu", cu, n + 1), self._ints("first", first, n), stride, width, n)
 
     def kv_write(self, cache: KvCache, k, v, table, cu, first):
         """k, v [rows, kv_heads, head_dim]: rows cu[b] .. cu[b+1] go to positions first[b] ... of sequence b (pages table[b])."""
-        if cache.device != self.device:
-            self._elsewhere("the cache", cache)
-        n, ks = self._heads("k", k, cache.kv_heads, cache.head_dim)
-        nv, vs = self._heads("v", v, cache.kv_heads, cache.head_dim)
-        if n != nv or k.dtype != v.dtype:
-            _refuse("k and v must be alike")
-        r = self._rows(table, cu, first)
-        rc = self._L.hipvoc_kv_write(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), n, self.stream)
-        if rc:
-            self._failed(rc)
+        _native.kv_write(self._h, self._index, cache, k, v, table, cu, first)
 
     def kv_read(self, cache: KvCache, table, cu, first, n_rows: int, dtype=None, out: Optional[Tuple] = None):
         """The inverse: (k, v) [n_rows, kv_heads, head_dim] in `dtype` (default: the cache's own), or into the two tensors of `out`;
         rows at or behind cu[-1] are left as they were."""
-        if cache.device != self.device:
-            self._elsewhere("the cache", cache)
-        if not 0 <= n_rows < 1 << 31:
-            _refuse(f"n_rows {n_rows} is negative or does not fit 32 bits")
-        heads, hd = cache.kv_heads, cache.head_dim
-        if out is None:
-            k = torch.empty((n_rows, heads, hd), dtype=dtype or cache.k.dtype, device=self.device)
-            v = torch.empty_like(k)
-            ks = vs = heads * hd
-        else:
-            k, v = out
-            n, ks = self._heads("k", k, heads, hd)
-            nv, vs = self._heads("v", v, heads, hd)
-            if n < n_rows or nv < n_rows or k.dtype != v.dtype:
-                _refuse("out must be two tensors of n_rows rows, alike in type")
-        r = self._rows(table, cu, first)
-        rc = self._L.hipvoc_kv_read(self._h, cache._p, k.data_ptr(), v.data_ptr(), ks, vs, _type(k), C.addressof(r), n_rows, self.stream)
-        if rc:
-            self._failed(rc)
-        return k, v
+        return _native.kv_read(self._h, self._index, cache, table, cu, first, n_rows, dtype, out)
 
     # ---- attention of one new token ------------------------------------------------------
     def attention(self, q, cache: KvCache, table, lens, scale: Optional[float] = None, window: int = 0, max_len: Optional[int] = None,
                   lse: bool = False, out=None):
         """q [seqs, heads, head_dim] over the lens[b] tokens of each sequence -> out like q; with lse=True also the log of the
         softmax's sum [seqs, heads] float32.  max_len: a bound on lens the host knows (default: all the table's pages hold)."""
-        if cache.device != self.device:
-            self._elsewhere("the cache", cache)
-        if q.dim() != 3:
-            _refuse("q must be [seqs, heads, head_dim]")
-        hd, heads = cache.head_dim, q.shape[1]
-        n, qs = self._heads("q", q, heads, hd)
-        tp, stride, width, nt = self._table(table)
-        if nt != n:
-            _refuse("table must have a row per sequence")
-        lp = self._ints("lens", lens, n)
-        if max_len is None:
-            max_len = width * cache.page
-        if not (0 <= max_len < 1 << 31 and 0 <= window < 1 << 31):
-            _refuse(f"max_len {max_len} or window {window} is negative or does not fit 32 bits")
-        if out is None:
-            out = torch.empty_like(q)
-            os_ = heads * hd
-        else:
-            no, os_ = self._heads("out", out, heads, hd)
-            if no != n or out.dtype != q.dtype:
-                _refuse("out must be like q")
-        sums = q.new_empty((n, heads), dtype=torch.float32) if lse else None
-        need = self._L.hipvoc_attention_workspace(cache._p, heads, n, max_len, window)
-        ws = lens.new_empty(need // 4) if need else None
-        rc = self._L.hipvoc_attention(
-            self._h, cache._p, q.data_ptr(), qs, out.data_ptr(), os_, sums.data_ptr() if lse else None, _type(q), heads, tp, stride, width, lp, n,
-            max_len, window, hd ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need, self.stream)
-        if rc:
-            self._failed(rc)
-        return (out, sums) if lse else out
+        return _native.attention(self._h, self._index, q, cache, table, lens, scale, window, max_len, lse, out)
 
     # ---- norm ----------------------------------------------------------------------------
     def add_rmsnorm(self, x, weight, residual=None, eps: float = 1e-6, quant: Optional[str] = None, group: int = 0):
         """x [rows, cols] (+ residual) -> (sum, y), or with quant "int8" / "e4m3" (sum, codes, scales [rows, cols / group]; group 0:
         one scale per row).  sum is None without a residual."""
-        rows, cols, xs = self._matrix("x", x)
-        act = x.dtype
-        t = _type(x)
-        if weight.dtype != act or weight.shape != (cols,) or not weight.is_contiguous():
-            _refuse("weight must be a contiguous [cols] of x's type")
-        if weight.device != self.device:
-            self._elsewhere("weight", weight)
-        rs, rp, total, sp = 0, None, None, None
-        if residual is not None:
-            rr, rc, rs = self._matrix("residual", residual)
-            if residual.dtype != act or rr != rows or rc != cols:
-                _refuse("residual must have x's type and shape")
-            total = torch.empty_like(x)
-            rp, sp = residual.data_ptr(), total.data_ptr()
-        if quant is None:
-            y, scales, ot, cp = torch.empty_like(x), None, t, None
-        elif quant == "int8" or quant == "e4m3":
-            if group and (group not in (32, 64, 128) or cols % group):
-                _refuse(f"group {group} must be 0, or 32, 64 or 128 and a divisor of cols {cols}")
-            ot = T_INT8 if quant == "int8" else T_E4M3
-            y = torch.empty_like(x, dtype=torch.int8 if ot == T_INT8 else torch.float8_e4m3fn)
-            scales = x.new_empty((rows, cols // group if group else 1), dtype=torch.float32)
-            cp = scales.data_ptr()
-        else:
-            _refuse("quant must be None, 'int8' or 'e4m3'")
-        rc = self._L.hipvoc_add_rmsnorm(self._h, x.data_ptr(), xs, rp, rs, weight.data_ptr(), sp, cols, y.data_ptr(), cols, cp, t, ot, group, eps, rows, cols,
-                                        self.stream)
-        if rc:
-            self._failed(rc)
-        return (total, y) if quant is None else (total, y, scales)
+        if quant is not None:
+            quant = T_INT8 if quant == "int8" else T_E4M3 if quant == "e4m3" else _refuse("quant must be None, 'int8' or 'e4m3'")
+        return _native.add_rmsnorm(self._h, self._index, x, weight, residual, eps, quant, group)
 
     # ---- 4-bit products ------------------------------------------------------------------
     def q4_matvec(self, codes, scales, x, mins=None, x_scale=None, dtype=None):
         """x [rows, n_in] times the 4-bit weights codes [n_out, n_in / 2] uint8, scales (mins) [n_out, n_in / group] float16 ->
         [rows, n_out].  int8 rows: x_scale [rows, n_in / group] or [rows, 1] float32, and `dtype` of the result (default float32)."""
-        cs, ss = codes.shape, scales.shape
-        if len(cs) != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
-            _refuse("codes must be a contiguous uint8 [n_out, n_in / 2]")
-        n_out, n_in = cs[0], cs[1] * 2
-        if n_out >> 31 or n_in >> 31:
-            _refuse(f"codes are {n_out} rows of {n_in}")
-        if len(ss) != 2 or ss[0] != n_out or scales.dtype != torch.float16 or not scales.is_contiguous() or ss[1] < 1 or n_in % ss[1]:
-            _refuse("scales must be a contiguous float16 [n_out, n_in / group]")
-        here, mp, xp = self.device, None, None
-        if mins is not None:
-            if mins.dtype != torch.float16 or mins.shape != ss or not mins.is_contiguous():
-                _refuse("mins must be like scales")
-            if mins.device != here:
-                self._elsewhere("mins", mins)
-            mp = mins.data_ptr()
-        if codes.device != here or scales.device != here:
-            self._elsewhere("codes or scales", codes if codes.device != here else scales)
-        rows, cols, xs = self._matrix("x", x)
-        if cols != n_in:
-            _refuse(f"x must have {n_in} columns")
-        xt, x_groups = _type(x), 0
-        if xt == T_INT8:
-            if x_scale is None or x_scale.dtype != torch.float32 or x_scale.dim() != 2 or x_scale.shape[0] != rows or not x_scale.is_contiguous():
-                _refuse("int8 rows need x_scale, a contiguous float32 [rows, n_in / group] or [rows, 1]")
-            if x_scale.device != here:
-                self._elsewhere("x_scale", x_scale)
-            x_groups, xp = x_scale.shape[1], x_scale.data_ptr()
-            out = dtype or torch.float32
-        elif x_scale is not None:
-            _refuse("only int8 rows have scales")
-        else:
-            out = dtype or x.dtype
-        y = x.new_empty((rows, n_out), dtype=out)
-        rc = self._L.hipvoc_q4_matvec(self._h, codes.data_ptr(), scales.data_ptr(), mp, n_out, n_in, n_in // ss[1], x.data_ptr(), xs, xt, xp, x_groups,
-                                      y.data_ptr(), n_out, _type(y), rows, self.stream)
-        if rc:
-            self._failed(rc)
-        return y
+        return _native.q4_matvec(self._h, self._index, codes, scales, x, mins, x_scale, dtype)
