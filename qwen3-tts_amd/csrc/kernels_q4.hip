@@ -98,38 +98,27 @@ template <int XT> struct XRow {
     }
 };
 
-static constexpr int Q4_WAVES = 8, Q4_HALVES = 2, Q4_GROUPS = 128;      // waves of a workgroup; of the wide kernel, on how many shares of a block's slabs; groups of a row whose scales are in LDS at a time
+static constexpr int Q4_WAVES = 8;                    // waves of a workgroup
+static constexpr int Q4_GROUPS = 128;                 // groups of a row whose scales are in LDS at a time
+static constexpr int Q4_AHEAD = 2;                    // slabs of codes a wave of q4_kernel has asked for
 
-// What a wave reads of one slab of 128 columns
-template <int XT, int RT> struct Slab {
-    u32x4 w[RT];
-    XRow<XT> x[4];
-};
-
-// Where a lane reads: its rows of the weights and of x.  Slab s is 64 bytes of codes and 128 values on.
-template <int XT, int RT> struct Rows {
-    const uint8_t *w[RT];
-    const char *x;
-};
+// x of a slab of 128 columns, as a wave reads it for itself: 16 rows at `row` (this lane's), eight columns from 8 (lane / 16) of every 32
 template <int XT> constexpr int x_bytes() { return XT == HIPVOC_T_F32 ? 4 : XT == HIPVOC_T_INT8 ? 1 : 2; }
-
-template <int XT, int RT>
-__device__ __forceinline__ void q4_load(const Q4Args &a, const Rows<XT, RT> &r, Slab<XT, RT> &b, int s, int lane) {
-    const int j = lane >> 4;
-    constexpr int XB = x_bytes<XT>();
-    const char *x = r.x + ((int64_t)s * 128 + 8 * j) * XB;
-    if (s * 128 + 128 <= a.n_in) {
+template <int XT> struct XSlab {
+    XRow<XT> x[4];
+    __device__ __forceinline__ void load(const Q4Args &a, const char *row, int s, int lane) {
+        constexpr int XB = x_bytes<XT>();
+        const char *at = row + ((int64_t)s * 128 + 8 * (lane >> 4)) * XB;
+        const int have = (a.n_in - s * 128) / 32;                                 // a group behind the last is not used: read the slab's first instead
 #pragma unroll
-        for (int t = 0; t < RT; t++) b.w[t] = __builtin_nontemporal_load((const u32x4 *)(r.w[t] + (int64_t)s * 64 + 16 * j));
-#pragma unroll
-        for (int c = 0; c < 4; c++) b.x[c].load(x + c * 32 * XB);
-    } else {                                                                      // a group behind the last is not used: read the slab's first instead
-        const int have = (a.n_in - s * 128) / 32;
-#pragma unroll
-        for (int t = 0; t < RT; t++) b.w[t] = __builtin_nontemporal_load((const u32x4 *)(r.w[t] + (int64_t)s * 64 + (j < have ? 16 * j : 0)));
-#pragma unroll
-        for (int c = 0; c < 4; c++) b.x[c].load(x + (c < have ? c : 0) * 32 * XB);
+        for (int c = 0; c < 4; c++) x[c].load(at + (have >= 4 || c < have ? c : 0) * 32 * XB);
     }
+};
+// Slab s of this lane's rows of the weights
+template <int RT> __device__ __forceinline__ void q4_codes(const Q4Args &a, const uint8_t *const (&rows)[RT], u32x4 (&w)[RT], int s, int lane) {
+    const int j = lane >> 4, at = s * 64 + (s * 128 + 32 * j < a.n_in ? 16 * j : 0);
+#pragma unroll
+    for (int t = 0; t < RT; t++) w[t] = __builtin_nontemporal_load((const u32x4 *)(rows[t] + at));
 }
 
 // sc: (scale, least value), two f16, of the slab's first group for this lane's row of tile 0; tile t is t * 16 rows of `stride` further on.
@@ -317,35 +306,47 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void q4_kernel(Q4Args a, int kw) {
     h16x2 *scales = (h16x2 *)(lds + (INT8 ? held * 64 : 0));
     float *red = (float *)lds;                                                    // [kw][16][wg_rows + 1]
     f32x4 out[RT] = {};
-    Slab<XT, RT> cur, next;
-    Rows<XT, RT> rows;
+    XSlab<XT> cur, next;
+    u32x4 w[Q4_AHEAD][RT];                                                        // codes of the next slabs, each asked for again once used
+    const uint8_t *rows[RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) rows.w[t] = a.codes + (int64_t)min(n0 + row0 + 16 * t + r16, a.n_out - 1) * (a.n_in / 2);
-    rows.x = (const char *)a.x + min(m0 + r16, a.n_rows - 1) * a.x_stride * x_bytes<XT>();
-    if (part < slabs) q4_load<XT, RT>(a, rows, cur, part, lane);
+    for (int t = 0; t < RT; t++) rows[t] = a.codes + (int64_t)min(n0 + row0 + 16 * t + r16, a.n_out - 1) * (a.n_in / 2);
+    const char *x = (const char *)a.x + min(m0 + r16, a.n_rows - 1) * a.x_stride * x_bytes<XT>();
+#pragma unroll
+    for (int u = 0; u < Q4_AHEAD; u++)
+        if (part + u * kw < slabs) q4_codes<RT>(a, rows, w[u], part + u * kw, lane);
+    if (part < slabs) cur.load(a, x, part, lane);
+    // a share of the scales' groups is a multiple of Q4_AHEAD * kw slabs, or the row's rest
     for (int g0 = 0; g0 < groups; g0 += Q4_GROUPS) {
         if (g0) __syncthreads();
         q4_stage_scales<XT, MINS>(a, scales, x_scales, n0, m0, wg_rows, groups, g0, stride);
         __syncthreads();
         const int last = min(slabs, (g0 + Q4_GROUPS) * G / 128);
-        for (int i = g0 * G / 128 + part; i < last; i += kw) {
-            if (i + kw < slabs) q4_load<XT, RT>(a, rows, next, i + kw, lane);
-            const int g = i * 128 / G - g0;
-            q4_use<XT, G, MINS, RT>(a, cur.w, [&](int c, auto *o) { cur.x[c].parts(o); }, i * 128, &scales[(row0 + r16) * stride + g], stride, INT8 ? (const f32x4 *)&x_scales[g][4 * j] : nullptr, out);
-            cur = next;
+        for (int i0 = g0 * G / 128 + part; i0 < last; i0 += Q4_AHEAD * kw) {
+#pragma unroll
+            for (int u = 0; u < Q4_AHEAD; u++) {
+                const int i = i0 + u * kw;
+                if (i >= last) break;
+                if (i + kw < slabs) next.load(a, x, i + kw, lane);
+                const int g = i * 128 / G - g0;
+                q4_use<XT, G, MINS, RT>(a, w[u], [&](int c, auto *o) { cur.x[c].parts(o); }, i * 128, &scales[(row0 + r16) * stride + g], stride, INT8 ? (const f32x4 *)&x_scales[g][4 * j] : nullptr, out);
+                if (i + Q4_AHEAD * kw < slabs) q4_codes<RT>(a, rows, w[u], i + Q4_AHEAD * kw, lane);
+                cur = next;
+            }
         }
     }
     q4_finish<XT, RT>(a, out, red, kw, part, row0, wg_rows, n0, m0);
 }
 
 // Many rows of weights: x goes through LDS.  A matrix operand's 16 rows of x are 16 lines for one load of 1 KB, and the cache serves a line in about
-// four cycles whatever is taken of it: read by every wave for itself, x cost more than the weights (79 / 54 / 47 us for 1 / 2 / 4 tiles per
-// read of x; 65536 x 4096, 16 rows).  Here all waves read it along its rows, a block of BS slabs ahead, and lay it down in operand order.
-template <int XT, int G, bool MINS, int RT>
+// four cycles whatever is taken of it: read by every wave for itself, x costs more than the weights (see q4_rt).  Here all waves read it along its rows, a block of BS slabs ahead, and lay it down in operand order.
+// KW waves share a block's slabs, so the workgroup has 16 RT Q4_WAVES / KW rows.
+template <int XT, int KW> constexpr int q4_block() { return XT == HIPVOC_T_F32 ? KW : 8; }         // slabs of a block
+template <int XT, int G, bool MINS, int RT, int KW>
 __global__ __launch_bounds__(64 * Q4_WAVES) void q4_wide_kernel(Q4Args a) {
-    constexpr int kw = Q4_HALVES;
+    constexpr int kw = KW;
     constexpr bool INT8 = XT == HIPVOC_T_INT8;
-    constexpr int BS = XT == HIPVOC_T_F32 ? 2 : 8, MINE = BS / kw, P = XRow<XT>::P, UNITS = BS * 256 / (64 * Q4_WAVES);     // slabs of a block, of them a wave's own; what a thread lays down of x
+    constexpr int BS = q4_block<XT, KW>(), MINE = BS / KW, P = XRow<XT>::P, UNITS = BS * 256 / (64 * Q4_WAVES);     // of a block's slabs a wave's own; what a thread lays down of x
     typedef typename std::conditional<INT8, long, u32x4>::type op_t;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = Q4_WAVES, r16 = lane & 15, j = lane >> 4;
@@ -381,15 +382,10 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void q4_wide_kernel(Q4Args a) {
     const uint8_t *rows[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) rows[t] = a.codes + (int64_t)min(n0 + row0 + 16 * t + r16, a.n_out - 1) * (a.n_in / 2);
-    const auto load = [&](u32x4 (&w)[RT], int s) {
-        const int at = s * 64 + (s * 128 + 32 * j < a.n_in ? 16 * j : 0);
-#pragma unroll
-        for (int t = 0; t < RT; t++) w[t] = __builtin_nontemporal_load((const u32x4 *)(rows[t] + at));
-    };
     fetch(0);
 #pragma unroll
     for (int i = 0; i < MINE; i++)
-        if (part + i * kw < slabs) load(w[i], part + i * kw);
+        if (part + i * kw < slabs) q4_codes<RT>(a, rows, w[i], part + i * kw, lane);
     for (int s0 = 0; s0 < slabs; s0 += BS) {
         const int g0 = s0 * 128 / G;
         if (s0) __syncthreads();                                                  // the last block is used up
@@ -407,20 +403,21 @@ __global__ __launch_bounds__(64 * Q4_WAVES) void q4_wide_kernel(Q4Args a) {
 #pragma unroll
                 for (int p = 0; p < P; p++) o[p] = xs[(c * P + p) * 64 + (r16 ^ (4 * c + j))];
             }, s * 128, &scales[(row0 + r16) * stride + g], stride, INT8 ? (const f32x4 *)&x_scales[g][4 * j] : nullptr, out);
-            if (s + BS < slabs) load(w[i], s + BS);
+            if (s + BS < slabs) q4_codes<RT>(a, rows, w[i], s + BS, lane);
         }
     }
     q4_finish<XT, RT>(a, out, red, kw, part, row0, wg_rows, n0, m0);
 }
 
-template <int XT> static size_t q4_wide_lds(int rt, int groups) {
-    return (XT == HIPVOC_T_F32 ? 24576 : XT == HIPVOC_T_INT8 ? 16384 : 32768) + q4_lds(XT == HIPVOC_T_INT8, 16 * rt * Q4_WAVES / Q4_HALVES, groups, Q4_HALVES);
+template <int XT, int RT, int KW> static size_t q4_wide_lds(int groups) {
+    const size_t x = (size_t)q4_block<XT, KW>() * 256 * (XT == HIPVOC_T_INT8 ? 8 : 16 * XRow<XT>::P);
+    return x + q4_lds(XT == HIPVOC_T_INT8, 16 * RT * Q4_WAVES / KW, groups, KW);
 }
 static constexpr size_t Q4_LDS = 160 * 1024;
-template <int XT, int G, bool MINS, int RT> static hipError_t q4_wide(const Q4Args &a, hipStream_t s) {
-    constexpr int rows = 16 * RT * Q4_WAVES / Q4_HALVES;
-    const size_t lds = q4_wide_lds<XT>(RT, a.n_in / G);
-    const auto kernel = q4_wide_kernel<XT, G, MINS, RT>;
+template <int XT, int G, bool MINS, int RT, int KW> static hipError_t q4_wide(const Q4Args &a, hipStream_t s) {
+    constexpr int rows = 16 * RT * Q4_WAVES / KW;
+    const size_t lds = q4_wide_lds<XT, RT, KW>(a.n_in / G);
+    const auto kernel = q4_wide_kernel<XT, G, MINS, RT, KW>;
     if (lds > 65536) {                                                            // over the default of a launch: said once per device
         static std::atomic<bool> said[64];
         int dev = 0;
@@ -434,28 +431,27 @@ template <int XT, int G, bool MINS, int RT> static hipError_t q4_wide(const Q4Ar
     kernel<<<dim3((a.n_out + rows - 1) / rows, (a.n_rows + 15) / 16), 64 * Q4_WAVES, lds, s>>>(a);
     return hipGetLastError();
 }
-// Which kernel, by the number of weight rows (4096 columns, groups of 64, 1 / 16 rows of x; us).  A workgroup of the wide kernel is slow by itself (it
-// takes 64 RT rows through four blocks), so it needs enough rows to fill 256 CUs:
-//    8192 rows: direct 8.7 / 13    wide<1> 15 / 15        16384: direct 16 / 23    wide<1> 16 / 16
-//   32768:      direct 29 / 43     wide<1> 22 / 23   wide<2> 22 / 23   wide<4> 33 / 34
-//   65536:      direct 56 / 84     wide<1> 41 / 44   wide<2> 43 / 45   wide<4> 37 / 39
-// 32-bit rows (three matrix instructions for one, blocks of two slabs), 4 rows of x: 16384: direct<1> 35, direct<2> 22, wide<2> 37; 65536: direct<2> 83,
-// wide<2> 56, wide<4> 54.
+// Which kernel, by the number of weight rows.  A workgroup is slow by itself (it goes through all columns: scales, codes, sums), so one workgroup per
+// CU with as few tiles as that takes is best while 256 of them can have all rows; beyond, x is better shared in LDS.  us, 2 rows of x in bf16, 4096
+// columns, groups of 64 / 16 rows, 1024 columns / 2 rows in f32, 2048 columns (RT for q4_kernel, RT x KW for q4_wide_kernel):
+//    rows    1                  2                  4                  2 x 4              4 x 2
+//    5000    8.7 / 5.7 / 10.5   8.5 / 5.2 / 7.7    12 / 6.8 / 10      14 / 6.0 / 12      31 / 13 / 26
+//   12288    13 / 8.2 / 15      15 / 8.8 / 14      12 / 6.9 / 10      14 / 6.2 / 12      32 / 13 / 27
+//   24576    23 / 15 / 28       22 / 13 / 21       23 / 12 / 19       21 / 8.3 / 17      33 / 14 / 27
+//   65536    56 / 36 / 72       56 / 32 / 52       46 / 24 / 38       40 / 15 / 32       36 / 15 / 28
 template <int XT, int G, bool MINS> static hipError_t q4_rt(const Q4Args &a, hipStream_t s) {
     const int slabs = (a.n_in + 127) / 128, kw = slabs < Q4_WAVES ? slabs : Q4_WAVES;
     const auto direct = [&](int rt, auto kernel) {
         kernel<<<dim3((a.n_out + 16 * rt - 1) / (16 * rt), (a.n_rows + 15) / 16), 64 * kw, q4_lds(XT == HIPVOC_T_INT8, 16 * rt, a.n_in / G, kw), s>>>(a, kw);
         return hipGetLastError();
     };
-    if constexpr (XT == HIPVOC_T_F32) {
-        if (a.n_out >= 32768) return q4_wide<XT, G, MINS, 2>(a, s);
-        if (a.n_out >= 8192) return direct(2, q4_kernel<XT, G, MINS, 2>);
-    } else {
-        // 16-bit rows of over 126 groups: their scales and x do not fit the LDS beside each other with 256 rows
-        if (a.n_out >= 65536 && q4_wide_lds<XT>(4, a.n_in / G) <= Q4_LDS) return q4_wide<XT, G, MINS, 4>(a, s);
-        if (a.n_out >= 16384) return q4_wide<XT, G, MINS, 1>(a, s);
-    }
-    return direct(1, q4_kernel<XT, G, MINS, 1>);
+    const int64_t rows = (int64_t)a.n_out * ((a.n_rows + 15) / 16);              // the weights are gone through once for every 16 rows of x
+    if (rows <= 4096) return direct(1, q4_kernel<XT, G, MINS, 1>);
+    if (rows <= 8192) return direct(2, q4_kernel<XT, G, MINS, 2>);
+    if (rows <= 16384) return direct(4, q4_kernel<XT, G, MINS, 4>);
+    // 16-bit rows of over 126 groups: the scales of 256 rows and x do not fit the LDS beside each other
+    if (rows >= 65536 && q4_wide_lds<XT, 4, 2>(a.n_in / G) <= Q4_LDS) return q4_wide<XT, G, MINS, 4, 2>(a, s);
+    return q4_wide<XT, G, MINS, 2, 4>(a, s);
 }
 template <int XT, int G> static hipError_t q4_mins(const Q4Args &a, hipStream_t s) { return a.mins ? q4_rt<XT, G, true>(a, s) : q4_rt<XT, G, false>(a, s); }
 template <int XT> static hipError_t q4_group(const Q4Args &a, hipStream_t s) {

@@ -637,8 +637,11 @@ def test_q4_matvec_larger(ops, act, m, n, k):
     check_q4(ops, n, k, 32, False, rnd((m, k), ACT[act], 2), seed=4)
 
 
-# the kernels for many weight rows: from 16384 and 65536 of them (32-bit rows: 8192 and 32768)
+# more weight rows than a tile per CU: other kernels over 4096, 8192 and 16384 of them (counted for every 16 rows of x) and from 65536
 @pytest.mark.parametrize("act,n,group,mult,mins,m", [
+    ("bf16", 4097, 64, 9, True, 3), ("f16", 8190, 32, 131, False, 1), ("f32", 5003, 128, 3, True, 16), ("int8", 8192, 32, 35, True, 5),
+    ("bf16", 8193, 32, 260, False, 2), ("f16", 16384, 64, 19, True, 16), ("f32", 9001, 32, 130, True, 2), ("int8", 12345, 64, 21, False, 9),
+    ("bf16", 2050, 64, 17, True, 40), ("f16", 300, 128, 40, False, 900), ("int8", 1000, 32, 33, True, 300), ("f32", 2049, 32, 17, False, 70),
     ("bf16", 16384, 64, 5, True, 3), ("f16", 16390, 32, 33, False, 17), ("bf16", 65541, 128, 3, True, 1), ("f16", 65536, 64, 18, False, 16),
     ("bf16", 65537, 32, 40, True, 2), ("bf16", 16385, 32, 131, True, 5), ("f16", 65540, 32, 128, True, 2), ("bf16", 65536, 32, 123, False, 1),
     ("f16", 65536, 32, 125, False, 33), ("bf16", 16384, 32, 1, True, 1), ("f32", 8192, 64, 9, True, 2), ("f32", 8199, 32, 130, False, 1),
