@@ -111,7 +111,7 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
  * rounding.  sum may be x or residual themselves (same stride); y overlaps no input and not sum.
  * out_dtype = dtype: y [rows][cols] in the act type.  INT8 / E4M3: y holds codes (bytes) and scales [rows][cols/group] f32,
  * one per `group` columns (32, 64, 128, or 0 for one per row; group divides cols), code and scale as in the cache.
- * Fewer than 2^22 rows; any cols from 1 to 2^20, any alignment: rows that are no multiple of 8 long or not 16-byte aligned take a slower kernel.
+ * Fewer than 2^22 rows; any cols from 1 to 2^20, any alignment.
  */
 int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
                        const void *weight, void *sum, int64_t sum_stride, void *y, int64_t y_stride, float *scales,

@@ -15,23 +15,51 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// OUT == ACT: y in the act type, else codes.  TH threads (64, 256 or 1024) have a row; a workgroup has max(TH, 256) threads.
-template <int ACT, int OUT, int TH, int NV>
+// Eight values anywhere (ODD: a row whose length, stride or place is no multiple of 16 bytes; global memory is read and written in up to 16 bytes at any
+// alignment)
+template <int T, bool ODD> __device__ __forceinline__ void load_vec(const typename Store<T>::type *p, float *f) {
+    if constexpr (!ODD) {
+        load8<T>(p, f);
+    } else {
+        Raw8<T> raw;
+        __builtin_memcpy(&raw, p, sizeof raw);
+        load8<T>(&raw, f);
+    }
+}
+template <int T, bool ODD> __device__ __forceinline__ void store_vec(typename Store<T>::type *p, const float *f) {
+    if constexpr (!ODD) {
+        store8<T>(p, f);
+    } else {
+        Raw8<T> raw;
+        store8<T>(&raw, f);
+        __builtin_memcpy(p, &raw, sizeof raw);
+    }
+}
+template <bool ODD> __device__ __forceinline__ void store_codes(uint8_t *p, u32x2 c) {
+    if constexpr (!ODD) *(u32x2 *)p = c;
+    else __builtin_memcpy(p, &c, 8);
+}
+
+// OUT == ACT: y in the act type, else codes.  TH threads (64, 256 or 1024) have a row; a workgroup has max(TH, 256) threads.  ODD: the last vector of a
+// row that is no multiple of 8 long ends with the row; what it has in common with the one before counts once, is read before anything is
+// written, and is written twice alike (8192 x 2047 in bf16: 26 us; element by element, 45).
+template <int ACT, int OUT, int TH, int NV, bool ODD>
 __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormArgs a) {
     constexpr int ROWS = TH < 256 ? 256 / TH : 1, NWAVE = TH / 64;
     typedef typename Store<ACT>::type act_t;
     __shared__ float sh[NWAVE > 1 ? NWAVE : 1];
     __shared__ unsigned sh_top[NWAVE > 1 ? NWAVE : 1];
-    const int t = threadIdx.x % TH, row = blockIdx.x * ROWS + threadIdx.x / TH, vecs = a.cols / 8;
+    const int t = threadIdx.x % TH, row = blockIdx.x * ROWS + threadIdx.x / TH;
     if (ROWS > 1 && row >= a.rows) return;                      // a wave's own row: no barrier follows
-    const act_t *x = (const act_t *)a.x + row * a.x_stride, *r = (const act_t *)a.residual + row * a.residual_stride;
+    const act_t *x = (const act_t *)a.x + row * a.x_stride, *r = (const act_t *)a.residual + row * a.residual_stride, *weight = (const act_t *)a.weight;
+    const auto has = [&](int v) { return (v * TH + t) * 8 < a.cols; };
+    const auto at = [&](int v) { return ODD ? min((v * TH + t) * 8, a.cols - 8) : (v * TH + t) * 8; };       // where this thread's vector v stands
     float s[NV][8], w[NV][8], sq = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-        const int i = v * TH + t;
-        if (i < vecs) {
-            load8<ACT>(x + i * 8, s[v]);
-            load8<ACT>((const act_t *)a.weight + i * 8, w[v]);
+        if (has(v)) {
+            load_vec<ACT, ODD>(x + at(v), s[v]);
+            load_vec<ACT, ODD>(weight + at(v), w[v]);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) s[v][e] = w[v][e] = 0.f;
@@ -40,10 +68,9 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
     if (a.residual) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const int i = v * TH + t;
-            if (i < vecs) {
+            if (has(v)) {
                 float b[8];
-                load8<ACT>(r + i * 8, b);
+                load_vec<ACT, ODD>(r + at(v), b);
 #pragma unroll
                 for (int e = 0; e < 8; e++) s[v][e] += b[e];
             }
@@ -52,7 +79,10 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
 #pragma unroll
     for (int v = 0; v < NV; v++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) sq = fmaf(s[v][e], s[v][e], sq);
+        for (int e = 0; e < 8; e++) {
+            const float one = ODD && at(v) + e < (v * TH + t) * 8 ? 0.f : s[v][e];
+            sq = fmaf(one, one, sq);
+        }
     }
     sq = wave_sum(sq);
     if constexpr (NWAVE > 1) {
@@ -66,15 +96,14 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
     unsigned top = 0;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-        const int i = v * TH + t;
-        if (a.sum && i < vecs) store8<ACT>((act_t *)a.sum + row * a.sum_stride + i * 8, s[v]);
+        if (a.sum && has(v)) store_vec<ACT, ODD>((act_t *)a.sum + row * a.sum_stride + at(v), s[v]);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             s[v][e] = s[v][e] * rs * w[v][e];
             if constexpr (OUT != ACT) top = amax_bits(top, s[v][e]);
         }
         if constexpr (OUT == ACT) {
-            if (i < vecs) store8<ACT>((act_t *)a.y + row * a.y_stride + i * 8, s[v]);
+            if (has(v)) store_vec<ACT, ODD>((act_t *)a.y + row * a.y_stride + at(v), s[v]);
         }
     }
     if constexpr (OUT != ACT) {
@@ -92,11 +121,10 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
             if (t == 0) a.scales[row] = scale;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
-                const int i = v * TH + t;
-                if (i < vecs) *(u32x2 *)(y + i * 8) = code.eight(s[v]);
+                if (has(v)) store_codes<ODD>(y + at(v), code.eight(s[v]));
             }
         } else {
-            // a group is 4, 8 or 16 neighbouring lanes of one vector index (TH is a multiple of 16)
+            // a group is 4, 8 or 16 neighbouring lanes of one vector index (TH is a multiple of 16), and a row whole groups
             const int lanes = a.group / 8;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
@@ -105,8 +133,8 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
 #pragma unroll
                 for (int e = 0; e < 8; e++) g = amax_bits(g, s[v][e]);
                 const float scale = scale8<OUT>(__uint_as_float(amax_lanes(g, lanes)));
-                if (i < vecs) {
-                    *(u32x2 *)(y + i * 8) = Coder<OUT>(scale).eight(s[v]);
+                if (has(v)) {
+                    store_codes<ODD>(y + i * 8, Coder<OUT>(scale).eight(s[v]));
                     if (i % lanes == 0) a.scales[(int64_t)row * (a.cols / a.group) + i / lanes] = scale;
                 }
             }
@@ -114,8 +142,8 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH) void add_rmsnorm_kernel(NormAr
     }
 }
 
-// Any length and alignment: a workgroup per row, one value at a time.  s is made anew in every pass, and the stored sum may be x or the
-// residual: it is written last, behind a barrier where another thread may still read its place.
+// Rows under 8 or over 32768 values: a workgroup per row, one value at a time.  s is made anew in every pass, and the stored sum may be x or the residual: it is
+// written last, behind a barrier where another thread may still read its place.
 template <int ACT, int OUT>
 __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(NormArgs a) {
     typedef typename Store<ACT>::type act_t;
@@ -158,24 +186,26 @@ __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(NormArgs a) {
     }
 }
 
-template <int ACT, int OUT, int TH, int NV> static void norm_go(const NormArgs &a, hipStream_t s) {
-    constexpr int ROWS = TH < 256 ? 256 / TH : 1;
-    add_rmsnorm_kernel<ACT, OUT, TH, NV><<<(a.rows + ROWS - 1) / ROWS, TH < 256 ? 256 : TH, 0, s>>>(a);
+template <int ACT, int OUT, int TH, int NV> static void norm_go(const NormArgs &a, bool odd, hipStream_t s) {
+    constexpr int ROWS = TH < 256 ? 256 / TH : 1, THREADS = TH < 256 ? 256 : TH;
+    const int blocks = (a.rows + ROWS - 1) / ROWS;
+    if (odd) add_rmsnorm_kernel<ACT, OUT, TH, NV, true><<<blocks, THREADS, 0, s>>>(a);
+    else add_rmsnorm_kernel<ACT, OUT, TH, NV, false><<<blocks, THREADS, 0, s>>>(a);
 }
 template <int ACT, int OUT> static hipError_t norm_out(const NormArgs &a, hipStream_t s) {
     constexpr int A = ACT == HIPVOC_T_F32 ? 4 : 2;
-    auto odd = [](const void *p, int64_t stride, int size) { return (((uintptr_t)p) | (uint64_t)(stride * size)) & 15; };
-    bool any = a.cols % 8 || odd(a.x, a.x_stride, A) || odd(a.weight, 0, A) || (a.residual && odd(a.residual, a.residual_stride, A)) ||
-               (a.sum && odd(a.sum, a.sum_stride, A));
-    any = any || (OUT == ACT ? odd(a.y, a.y_stride, A) != 0 : ((((uintptr_t)a.y) | (uint64_t)a.y_stride) & 7) != 0);
-    const int vecs = a.cols / 8;
-    if (any || vecs > 4096) add_rmsnorm_any_kernel<ACT, OUT><<<a.rows, 256, 0, s>>>(a);
-    else if (vecs <= 64) norm_go<ACT, OUT, 64, 1>(a, s);
-    else if (vecs <= 128) norm_go<ACT, OUT, 64, 2>(a, s);
-    else if (vecs <= 256) norm_go<ACT, OUT, 256, 1>(a, s);
-    else if (vecs <= 512) norm_go<ACT, OUT, 256, 2>(a, s);
-    else if (vecs <= 1024) norm_go<ACT, OUT, 256, 4>(a, s);
-    else norm_go<ACT, OUT, 1024, 4>(a, s);
+    auto off = [](const void *p, int64_t stride, int size) { return (((uintptr_t)p) | (uint64_t)(stride * size)) & 15; };
+    bool odd = a.cols % 8 || off(a.x, a.x_stride, A) || off(a.weight, 0, A) || (a.residual && off(a.residual, a.residual_stride, A)) ||
+               (a.sum && off(a.sum, a.sum_stride, A));
+    odd = odd || (OUT == ACT ? off(a.y, a.y_stride, A) != 0 : ((((uintptr_t)a.y) | (uint64_t)a.y_stride) & 7) != 0);
+    const int vecs = (a.cols + 7) / 8;
+    if (a.cols < 8 || vecs > 4096) add_rmsnorm_any_kernel<ACT, OUT><<<a.rows, 256, 0, s>>>(a);
+    else if (vecs <= 64) norm_go<ACT, OUT, 64, 1>(a, odd, s);
+    else if (vecs <= 128) norm_go<ACT, OUT, 64, 2>(a, odd, s);
+    else if (vecs <= 256) norm_go<ACT, OUT, 256, 1>(a, odd, s);
+    else if (vecs <= 512) norm_go<ACT, OUT, 256, 2>(a, odd, s);
+    else if (vecs <= 1024) norm_go<ACT, OUT, 256, 4>(a, odd, s);
+    else norm_go<ACT, OUT, 1024, 4>(a, odd, s);
     return hipGetLastError();
 }
 template <int ACT> static hipError_t norm_act(const NormArgs &a, hipStream_t s) {

@@ -563,9 +563,9 @@ def test_add_rmsnorm_special_rows(ops):
 
 
 def test_add_rmsnorm_in_place(pkg, ops):
-    """The C entry point may put the sum over x or over the residual, on both kernels."""
+    """The C entry point may put the sum over x or over the residual, whatever kernel the length takes."""
     L, p = ops._L, lambda t: t.data_ptr()  # noqa: E731
-    for cols in (256, 250):
+    for cols in (256, 250, 5, 8, 9, 1023, 1027, 2047, 4099, 8191, 32763, 33001):
         for quant in (2, 3):                                    # bf16 out, int8 out
             x, r, w = rnd((5, cols), torch.bfloat16, 8).cuda(), rnd((5, cols), torch.bfloat16, 9).cuda(), rnd((cols,), torch.bfloat16, 10).cuda()
             want = ops.add_rmsnorm(x, w, r, eps=1e-5, quant=None if quant == 2 else "int8")
@@ -578,6 +578,27 @@ def test_add_rmsnorm_in_place(pkg, ops):
                 assert rc == 0
                 assert torch.equal((a, b)[into], want[0]) and torch.equal(y, want[1])
     ops.sync()
+
+
+@pytest.mark.parametrize("cols", [1, 7, 8, 9, 15, 63, 513, 1025, 2051, 4097, 8195, 32761])
+@pytest.mark.parametrize("quant", [None, "int8"])
+def test_add_rmsnorm_writes_its_rows_alone(ops, cols, quant):
+    """Odd rows inside wider ones, at odd places: what lies between and behind them is left as it was."""
+    L, p, rows, wide = ops._L, lambda t: t.data_ptr(), 3, cols + 5  # noqa: E731
+    x, r, w = [rnd((n, cols), torch.bfloat16, 30 + n).cuda() for n in (rows, rows, 1)]
+    w = w[0].contiguous()
+    want = ops.add_rmsnorm(x, w, r, eps=1e-5, quant=quant)
+    out = torch.bfloat16 if quant is None else torch.int8
+    sums, y = torch.full((rows * wide + 9,), 7.0, dtype=torch.bfloat16, device="cuda"), torch.full((rows * wide + 9,), 7, dtype=out, device="cuda")
+    s = torch.empty((rows, 1), device="cuda")
+    rc = L.hipvoc_add_rmsnorm(ops._h, p(x), cols, p(r), cols, p(w), p(sums[3:]), wide, p(y[5:]), wide, None if quant is None else p(s), 2, 2 if quant is None else 3, 0,
+                              1e-5, rows, cols, ops.stream)
+    assert rc == 0
+    ops.sync()
+    for flat, at, ref in ((sums, 3, want[0]), (y, 5, want[1])):
+        keep = torch.full((rows * wide + 9,), 7, dtype=flat.dtype, device="cuda")
+        keep[at:at + rows * wide].view(rows, wide)[:, :cols] = ref
+        assert torch.equal(flat, keep)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
