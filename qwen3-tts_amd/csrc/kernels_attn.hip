@@ -3,13 +3,13 @@
 // Mathematics: one pass over the keys with a running maximum m and sum l per query head (softmax in powers of two, s = q.k * scale *
 // log2(e)):  m' = max(m, s), l' = l 2^(m-m') + 2^(s-m'), o' = o 2^(m-m') + 2^(s-m') v.  States (m, l, o) of disjoint key sets join by
 // the same rule.
-// Bound: memory.  Every key and value row is read once for all query heads of its key head (16 of them; 4 for 32-bit activations).
+// Bound: memory.  Every key and value row is read once for all query heads of its key head (up to 16 of them; 4 on a 32-bit cache).
 // Split: n_seqs * kv_heads workgroups do not fill 256 CUs, and sequences differ in length.  So all the tiles of a call stand in one row and
-// every wave (32-bit activations: workgroup) has an equal share of it, wherever its ends fall (ops_index.hpp); the pieces of a sequence are
-// joined by a second kernel, without atomics: the order of every sum follows from the call's lengths.  Against a grid of fixed chunks: 128
-// sequences of 400 .. 2048 tokens in bf16 56.6 us (72), since the chip's dies got unequal chunks.  Up to 24 tiles (768 keys) a workgroup has a
-// sequence and key head to itself: 500 keys 10 us, cut 14.  8 KV heads, 128 values: 32768 tokens x 4 in bf16, 537 MB, 97 us (5.5 TB/s); in
-// 8 bits, 65536 tokens x 4, 566 MB, 110 us (5.1 TB/s).  32-bit activations: 544 MB of 32-bit cache 109 us, 272 MB of 8-bit cache 71 us.
+// every wave (32-bit caches: workgroup) has an equal share of it, wherever its ends fall (ops_index.hpp); the pieces of a sequence are
+// joined by a second kernel, without atomics: the order of every sum follows from the call's lengths.  A grid of fixed
+// chunks gave the chip's dies unequal ones: 32 sequences of up to 4095 tokens, 8 key heads of 128, 16 query heads in bf16 (272 MB) 72 us, so 55.5 us
+// (4.9 TB/s).  131071 tokens, 32 query heads in f16 (537 MB) 96 us, 5.6 TB/s; 64 sequences of up to 8192 in 8 bits (566 MB) 110 us, 5.1 TB/s.
+// 32-bit activations, 32 sequences of up to 4095: 544 MB of 32-bit cache 109 us; 8 bits 51 us, alike for 1 to 8 query heads per key head.
 #include "ops_device.h"
 
 namespace hipvoc {
@@ -150,13 +150,11 @@ __device__ __forceinline__ void attn_finish(const AttnArgs &a, const AttnPiece &
     }
 }
 
-// 32-bit activations: a wave reads rows of HD values with HD / 8 lanes each, U rows per lane in flight, and keeps HT query heads in registers.
-template <int ST, int HD, int HT>
+// 32-bit caches: a wave reads rows of HD values with HD / 8 lanes each, U rows per lane in flight, and keeps HT query heads in registers.
+template <int HD, int HT>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     constexpr int ACT = HIPVOC_T_F32;
     constexpr int LPR = HD / 8, KPS = 64 / LPR, U = 4, TILE = U * KPS, NW = 4;
-    typedef typename Store<ACT>::type act_t;
-    typedef typename Store<ST>::type st_t;
     __shared__ float sh_o[NW][HT][HD], sh_m[NW][HT], sh_l[NW][HT];
     __shared__ int sh_bad[NW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = (lane % LPR) * 8, kl = lane / LPR;
@@ -168,14 +166,14 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         for (int h = 0; h < HT; h++) {
             m[h] = -__builtin_inff();
             l[h] = 0.f;
-            load8<ACT>((const act_t *)a.q + seq * a.q_stride + (int64_t)min(h0 + h, h0 + nh - 1) * HD + d, q[h]);
+            load8<ACT>((const float *)a.q + seq * a.q_stride + (int64_t)min(h0 + h, h0 + nh - 1) * HD + d, q[h]);
 #pragma unroll
             for (int i = 0; i < 8; i++) o[h][i] = 0.f;
         }
         const int32_t *table = a.table + seq * a.table_stride;
         bool bad = false;
         for (int base = sp.from + wave * TILE; base < sp.to; base += NW * TILE) {
-            float k[U][8], v[U][8], ks[U], vs[U], s[HT][U];
+            float k[U][8], v[U][8], s[HT][U];
             bool in[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -185,14 +183,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
                 if (!page_ok(page, a.c.n_pages)) { bad = true; page = 0; }
                 const int in_page = kc & (a.c.page - 1);
                 const int64_t row = page * a.c.page_stride + ((int64_t)kvh * a.c.page + in_page) * HD + d;
-                load8<ST>((const st_t *)a.c.k + row, k[u]);
-                load8<ST>((const st_t *)a.c.v + row, v[u]);
-                ks[u] = vs[u] = 1.f;
-                if constexpr (ST != ACT) {
-                    const int64_t sc = ((int64_t)page * a.c.kv_heads + kvh) * a.c.page + in_page;
-                    ks[u] = a.c.k_scale[sc];
-                    vs[u] = a.c.v_scale[sc];
-                }
+                load8<ACT>((const float *)a.c.k + row, k[u]);
+                load8<ACT>((const float *)a.c.v + row, v[u]);
             }
 #pragma unroll
             for (int h = 0; h < HT; h++) {
@@ -203,7 +195,6 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) x = fmaf(q[h][i], k[u][i], x);
                     x = sum_lanes<LPR>(x);
-                    if constexpr (ST != ACT) x *= ks[u];
                     s[h][u] = in[u] ? x * a.scale_log2 : -__builtin_inff();
                     top = fmaxf(top, s[h][u]);
                 }
@@ -214,9 +205,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
                 for (int i = 0; i < 8; i++) o[h][i] *= old;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
+                    const float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
                     l[h] += p;
-                    if constexpr (ST != ACT) p = in[u] ? p * vs[u] : 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
                 }
@@ -253,14 +243,16 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// 16-bit activations, on the matrix cores.  A wave has tiles of 32 keys for up to 16 query heads:
+// 16-bit activations, and 32-bit ones on 8-bit caches, on the matrix cores.  A wave has tiles of 32 keys for up to 16 query heads:
 //   S^T = K Q^T   (rows = keys, columns = heads): a lane of (m = lane % 16, j = lane / 16) reads key rows as they lie, 16 bytes at a time.
 //                 Row m of half t is key 8 (m / 4) + 4 t + m % 4, so a lane's eight results are the scores of ONE head for the keys 8j .. 8j+7,
 //   O^T = V^T P^T (rows = values' columns, columns = heads): and these, rounded, are at once the right operand.  The left one needs a column
 //                 of V for eight keys: the lane reads HD/16 neighbouring columns of its eight keys' rows (whole rows across 16 lanes) and
 //                 turns them with one byte permutation per two values; row m of product i is column m HD/16 + i.
 // So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P goes into the product with V as two values of V's own type (bf16 for
-// 8-bit codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().
+// 8-bit codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().  A 32-bit q or weight is three bf16, exactly:
+// three matrix instructions for one, still under the time of an 8-bit row's loads (the vector ALU's rate bound 32-bit activations on 8-bit caches by its
+// conversions and, for over 4 query heads per key head, a second reading).
 // What is masked is read from a row that is not (so that no stale value, NaN or page number behind the last token matters).
 
 // four codes to two pairs of 16-bit values, exactly
@@ -284,6 +276,13 @@ template <bool F16> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f3
     if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
 }
+// two floats as the sums of three bf16 each, exactly: cut off (not rounded: nothing can overflow) after 8 significant bits
+__device__ __forceinline__ void thirds(float x, float y, unsigned &a, unsigned &b, unsigned &c) {
+    const float x0 = bf16_hi(__float_as_uint(x)), y0 = bf16_hi(__float_as_uint(y)), x1 = bf16_hi(__float_as_uint(x - x0)), y1 = bf16_hi(__float_as_uint(y - y0));
+    a = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);
+    b = __builtin_amdgcn_perm(__float_as_uint(y1), __float_as_uint(x1), 0x07060302);
+    c = __builtin_amdgcn_perm(__float_as_uint(y - y0 - y1), __float_as_uint(x - x0 - x1), 0x07060302);
+}
 // maximum over the four lanes of a head (lane % 16)
 __device__ __forceinline__ float max_of_head(float v) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -295,12 +294,14 @@ __device__ __forceinline__ float max_of_head(float v) {
 // Keys and values are read once: non-temporal loads (512 MB: 6.9 TB/s against 6.1).
 template <typename T> __device__ __forceinline__ T once(const T *p) { return __builtin_nontemporal_load(p); }
 
-// Waves per SIMD that the matrix kernels' registers have to leave room for: up to 168, and attn_stream_kernel has 158 .. 165 for head_dim 128.
-static constexpr int ATTN_WAVES = 3;
+// Waves per SIMD that the matrix kernels' registers have to leave room for: 3 with up to 168 registers, of which attn_stream_kernel has 158 .. 165 for
+// head_dim 128; three times q does not fit those.
+constexpr int attn_waves(int act) { return act == HIPVOC_T_F32 ? 2 : 3; }
 
 // The keys and values of one tile for one wave, and what they do to the state of its heads
 template <int ACT, int ST, int HD> struct AttnWave {
-    static constexpr bool CODED = ST != ACT, QF16 = ACT == HIPVOC_T_F16, PF16 = QF16 && !CODED;
+    static constexpr bool CODED = ST != ACT, WIDE = ACT == HIPVOC_T_F32, QF16 = ACT == HIPVOC_T_F16, PF16 = QF16 && !CODED;
+    static constexpr int QP = WIDE ? 3 : 1, P = WIDE ? 3 : 2;            // operands that are together q, and the weights
     static constexpr int NC = HD / 32, NV = HD / 16;                     // products of S per 16 keys, and of O
     static constexpr int KW = CODED ? HD / 64 : NC, VW = CODED ? HD / 64 : HD / 32;      // 16-byte words of a key row, dwords of a value row that a lane reads
     typedef typename Store<ACT>::type act_t;
@@ -309,7 +310,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
     // A tile: its first key, the keys seen, the key head, the sequence's pages
     struct Tile { int base, lo, hi, kvh; const int32_t *table; };
 
-    u32x4 q[NC], k[2][KW];
+    u32x4 q[QP][NC], k[2][KW];
     unsigned v[8][VW];
     f32x4 ks[2], vs[2], o[NV];
     float m, l;
@@ -332,7 +333,23 @@ template <int ACT, int ST, int HD> struct AttnWave {
         const int m16 = lane & 15, j = lane >> 4;
         const act_t *row = (const act_t *)a.q + seq * a.q_stride + (int64_t)(h0 + min(m16, nh - 1)) * HD;
 #pragma unroll
-        for (int i = 0; i < NC; i++) q[i] = *(const u32x4 *)(row + (CODED ? (i >> 1) * 64 + 16 * j + 8 * (i & 1) : 32 * i + 8 * j));
+        for (int i = 0; i < NC; i++) {
+            const act_t *at = row + (CODED ? (i >> 1) * 64 + 16 * j + 8 * (i & 1) : 32 * i + 8 * j);
+            if constexpr (WIDE) {
+                float f[8];
+                load8<ACT>(at, f);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    unsigned a, b, c;
+                    thirds(f[2 * e], f[2 * e + 1], a, b, c);
+                    q[0][i][e] = a;
+                    q[1][i][e] = b;
+                    q[2][i][e] = c;
+                }
+            } else {
+                q[0][i] = *(const u32x4 *)at;
+            }
+        }
         m = -__builtin_inff();
         l = 0.f;
 #pragma unroll
@@ -397,13 +414,16 @@ template <int ACT, int ST, int HD> struct AttnWave {
 #pragma unroll
                 for (int i = 0; i < KW; i++) {
                     const u32x2 a0 = widen4<ST, QF16>(k[t][i][0]), a1 = widen4<ST, QF16>(k[t][i][1]), a2 = widen4<ST, QF16>(k[t][i][2]), a3 = widen4<ST, QF16>(k[t][i][3]);
-                    acc = mfma32<QF16>((u32x4){a0[0], a0[1], a1[0], a1[1]}, q[2 * i], acc);
-                    acc = mfma32<QF16>((u32x4){a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], acc);
+#pragma unroll
+                    for (int p = 0; p < QP; p++) {
+                        acc = mfma32<QF16>((u32x4){a0[0], a0[1], a1[0], a1[1]}, q[p][2 * i], acc);
+                        acc = mfma32<QF16>((u32x4){a2[0], a2[1], a3[0], a3[1]}, q[p][2 * i + 1], acc);
+                    }
                 }
                 acc *= ks[t];
             } else {
 #pragma unroll
-                for (int i = 0; i < NC; i++) acc = mfma32<QF16>(k[t][i], q[i], acc);
+                for (int i = 0; i < NC; i++) acc = mfma32<QF16>(k[t][i], q[0][i], acc);
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) s[4 * t + r] = acc[r] * a.scale_log2;
@@ -419,7 +439,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
     // The running maximum and sum, and the weights as the right operand of the product with V: two operands whose sum they are, in the second what
     // the first leaves over.  One alone (bf16: 8 bits, f16: 11) would add as much error again as the rounding of the result, or a good part of it, and
     // the second product costs a tile 8 matrix instructions of 16 cycles and 20 vector ones, under the time of its loads: no time measured.
-    __device__ __forceinline__ void weights(const Tile &tl, const float (&s)[8], int lane, u32x4 (&pp)[2]) {
+    __device__ __forceinline__ void weights(const Tile &tl, const float (&s)[8], int lane, u32x4 (&pp)[P]) {
         const int j = lane >> 4;
         float top = m;
 #pragma unroll
@@ -451,7 +471,13 @@ template <int ACT, int ST, int HD> struct AttnWave {
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            if constexpr (PF16) {
+            if constexpr (WIDE) {
+                unsigned a, b, c;
+                thirds(p[2 * e], p[2 * e + 1], a, b, c);
+                pp[0][e] = a;
+                pp[1][e] = b;
+                pp[2][e] = c;
+            } else if constexpr (PF16) {
                 const unsigned hi = pack_f16(p[2 * e], p[2 * e + 1]);
                 const h16x2 most = __builtin_bit_cast(h16x2, hi);       // (cast from pp[0][e] itself the compiler takes pp[0][0])
                 pp[0][e] = hi;
@@ -462,7 +488,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
             }
         }
     }
-    __device__ __forceinline__ void values(const u32x4 (&pp)[2]) {
+    __device__ __forceinline__ void values(const u32x4 (&pp)[P]) {
         unsigned w[8][HD / 32];                                          // the value rows in 16 bits
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -483,7 +509,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
 #pragma unroll
             for (int e = 0; e < 4; e++) col[e] = __builtin_amdgcn_perm(w[2 * e + 1][i >> 1], w[2 * e][i >> 1], i & 1 ? 0x07060302 : 0x05040100);
 #pragma unroll
-            for (int p = 0; p < 2; p++) o[i] = mfma32<PF16>(col, pp[p], o[i]);
+            for (int p = 0; p < P; p++) o[i] = mfma32<PF16>(col, pp[p], o[i]);
         }
     }
     __device__ __forceinline__ float sum_of_head() const {
@@ -494,7 +520,7 @@ template <int ACT, int ST, int HD> struct AttnWave {
 
 // A workgroup per (sequence, pair), its four waves on every fourth tile
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256, ATTN_WAVES) void attn_whole_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, attn_waves(ACT)) void attn_whole_kernel(AttnArgs a) {
     typedef AttnWave<ACT, ST, HD> Wave;
     constexpr int NW = 4, NV = HD / 16;
     __shared__ __attribute__((aligned(16))) float sh_o[NW][16][HD + 4];
@@ -508,16 +534,36 @@ __global__ __launch_bounds__(256, ATTN_WAVES) void attn_whole_kernel(AttnArgs a)
     Wave w;
     w.start(a, seq, h0, nh, lane);
     typename Wave::Tile t = {sp.base + 32 * wave, sp.lo, sp.hi, kvh, a.table + seq * a.table_stride};
-    for (; t.base < sp.hi; t.base += 32 * NW) {
-        int pk = Wave::page_k(a, t, lane), pv = Wave::page_v(a, t, lane);
-        if (!page_ok(pk, a.c.n_pages) || !page_ok(pv, a.c.n_pages)) { bad = true; pk = pv = 0; }
+    if (t.base < sp.hi) {
+        const auto sound = [&](int page) {
+            if (page_ok(page, a.c.n_pages)) return page;
+            bad = true;
+            return 0;
+        };
+        const auto step = [&](typename Wave::Tile &x) { x.base += x.base + 32 * NW < sp.hi ? 32 * NW : 0; };
+        int pk = sound(Wave::page_k(a, t, lane)), pv = sound(Wave::page_v(a, t, lane));
         w.load_k(a, t, pk, pv, true, lane);
         w.load_v(a, t, pv, true, lane);
-        float s[8];
-        w.scores(a, t, s, lane);
-        u32x4 pp[2];
-        w.weights(t, s, lane, pp);
-        w.values(pp);
+        typename Wave::Tile next = t;
+        step(next);
+        int nk = Wave::page_k(a, next, lane), nv = Wave::page_v(a, next, lane);
+        for (;;) {                                                       // the next tile is on its way while one is worked on
+            const bool more = next.base > t.base;
+            float s[8];
+            w.scores(a, t, s, lane);
+            pk = sound(nk);
+            pv = sound(nv);
+            w.load_k(a, next, pk, pv, more, lane);
+            u32x4 pp[Wave::P];
+            w.weights(t, s, lane, pp);
+            w.values(pp);
+            if (!more) break;
+            w.load_v(a, next, pv, true, lane);
+            t = next;
+            step(next);
+            nk = Wave::page_k(a, next, lane);
+            nv = Wave::page_v(a, next, lane);
+        }
     }
     const float l = w.sum_of_head();
     const bool wave_bad = __any(bad);
@@ -543,7 +589,7 @@ __global__ __launch_bounds__(256, ATTN_WAVES) void attn_whole_kernel(AttnArgs a)
 // their way as soon as this one's are used up, its values likewise, and the pages of the one after that; at a piece's end only the state is
 // written and the next head's q read.
 template <int ACT, int ST, int HD>
-__global__ __launch_bounds__(256, ATTN_WAVES) void attn_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, attn_waves(ACT)) void attn_stream_kernel(AttnArgs a) {
     typedef AttnWave<ACT, ST, HD> Wave;
     constexpr int NV = HD / 16;
     __shared__ int64_t before[ATTN_MAX_SEQS + 1];
@@ -620,7 +666,7 @@ __global__ __launch_bounds__(256, ATTN_WAVES) void attn_stream_kernel(AttnArgs a
         float s[8];
         w.scores(a, cur.t, s, lane);
         w.load_k(a, next.t, sk, sv, left > 1, lane);
-        u32x4 pp[2];
+        u32x4 pp[Wave::P];
         w.weights(cur.t, s, lane, pp);
         w.values(pp);
         w.load_v(a, next.t, sv, left > 1, lane);
@@ -642,6 +688,7 @@ __global__ __launch_bounds__(256, ATTN_WAVES) void attn_stream_kernel(AttnArgs a
                     const int d = (4 * j + r) * NV;
                     if (all) {
                         if constexpr (NV == 8) store8<ACT>(out + d, y);
+                        else if constexpr (ACT == HIPVOC_T_F32) *(f32x4 *)(out + d) = (f32x4){y[0], y[1], y[2], y[3]};
                         else *(u32x2 *)(out + d) = ACT == HIPVOC_T_F16 ? (u32x2){pack_f16(y[0], y[1]), pack_f16(y[2], y[3])} : (u32x2){pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
                     } else {
 #pragma unroll
@@ -669,7 +716,7 @@ __global__ __launch_bounds__(256, ATTN_WAVES) void attn_stream_kernel(AttnArgs a
 
 // Joins the pieces of the pairs that were cut.  A pair's result is I = heads * head_dim / 4 quads; a workgroup has `per` of them (all the pair's, or
 // fewer where the pairs do not fill the card) and walks the pieces 256 / per at a time, each thread with a running state of its own; the
-// threads of a quad are joined through LDS.  A sequence without a tile has no piece: its result is written here.
+// threads of a quad are joined through LDS, by halves.  A sequence without a tile has no piece: its result is written here.
 template <int ACT, int HD, int H>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
     __shared__ __attribute__((aligned(16))) f32x4 sh_o[256];
@@ -690,34 +737,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
         slot0 = w0 + (int64_t)seq * a.heads + pair;
         n = (int)(w1 - w0) + 1;
     }
+    const int g = t / per;
     for (int first = blockIdx.z * per; first < quads; first += gridDim.z * per) {
-        const int quad = first + t % per, g = t / per, h = min(quad / (HD / 4), nh - 1), d = quad % (HD / 4) * 4;
+        const int quad = first + t % per, h = min(quad / (HD / 4), nh - 1), d = quad % (HD / 4) * 4;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float m = -__builtin_inff(), l = bad ? __builtin_nanf("") : 0.f;
-        if (g < groups) {
+        const auto join = [&](f32v2 ml, f32x4 v) {
+            const float top = fmaxf(m, ml[0]), safe = top == -__builtin_inff() ? 0.f : top;
+            const float f = __builtin_amdgcn_exp2f(m - safe), e = __builtin_amdgcn_exp2f(ml[0] - safe);      // a NaN is dropped by the maximum and kept by these
+            m = top;
+            l = l * f + ml[1] * e;
+            o = o * f + v * e;
+        };
 #pragma unroll 4
-            for (int c = g; c < n; c += groups) {
-                const f32v2 ml = *slot_ml<HD, H>(a, slot0 + c, h);
-                const f32x4 v = *(const f32x4 *)(slot_o<HD, H>(a, slot0 + c, h) + d);
-                const float top = fmaxf(m, ml[0]), safe = top == -__builtin_inff() ? 0.f : top;
-                const float f = __builtin_amdgcn_exp2f(m - safe), e = __builtin_amdgcn_exp2f(ml[0] - safe);      // a NaN is dropped by the maximum and kept by these
-                m = top;
-                l = l * f + ml[1] * e;
-                o = o * f + v * e;
+        for (int c = g; c < n; c += groups) join(*slot_ml<HD, H>(a, slot0 + c, h), *(const f32x4 *)(slot_o<HD, H>(a, slot0 + c, h) + d));
+        for (int half = groups / 2; half; half /= 2) {
+            if (g >= half && g < 2 * half) {
+                sh_o[t] = o;
+                sh_ml[t] = (f32v2){m, l};
             }
-            sh_o[t] = o;
-            sh_ml[t] = (f32v2){m, l};
+            __syncthreads();
+            if (g < half) join(sh_ml[t + half * per], sh_o[t + half * per]);
         }
-        __syncthreads();
         if (g == 0 && quad < quads) {
-            for (int i = 1; i < groups; i++) {
-                const f32v2 ml = sh_ml[i * per + t];
-                const float top = fmaxf(m, ml[0]), safe = top == -__builtin_inff() ? 0.f : top;
-                const float f = __builtin_amdgcn_exp2f(m - safe), e = __builtin_amdgcn_exp2f(ml[0] - safe);
-                m = top;
-                l = l * f + ml[1] * e;
-                o = o * f + sh_o[i * per + t] * e;
-            }
             const int64_t at = seq * a.out_stride + (int64_t)(h0 + h) * HD + d;
 #pragma unroll
             for (int i = 0; i < 4; i++) store1<ACT>(a.out, at + i, l == 0.f ? 0.f : bad ? l : o[i] / l);
@@ -729,7 +771,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int per) {
 
 template <int ACT, int ST, int HD, int H> static hipError_t attn_launch(const AttnArgs &a, hipStream_t s) {
     const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.heads;
-    if constexpr (ACT == HIPVOC_T_F32) attn_rows_kernel<ST, HD, H><<<a.workers ? (unsigned)a.workers : pairs, 256, 0, s>>>(a);
+    if constexpr (ST == HIPVOC_T_F32) attn_rows_kernel<HD, H><<<a.workers ? (unsigned)a.workers : pairs, 256, 0, s>>>(a);
     else if (a.workers) attn_stream_kernel<ACT, ST, HD><<<(a.workers + 3) / 4, 256, 0, s>>>(a);
     else attn_whole_kernel<ACT, ST, HD><<<pairs, 256, 0, s>>>(a);
     hipError_t e = hipGetLastError();
@@ -743,7 +785,7 @@ template <int ACT, int ST, int HD, int H> static hipError_t attn_launch(const At
     return e;
 }
 template <int ACT, int ST, int HD> static hipError_t attn_go(const AttnArgs &a, hipStream_t s) {
-    if constexpr (ACT == HIPVOC_T_F32) {
+    if constexpr (ST == HIPVOC_T_F32) {
         if (a.group == 1) return attn_launch<ACT, ST, HD, 1>(a, s);
         if (a.group == 2) return attn_launch<ACT, ST, HD, 2>(a, s);
         return attn_launch<ACT, ST, HD, 4>(a, s);

@@ -28,7 +28,7 @@ OPS_FN AttnSpan attn_span(int n, int max_len, int window) {
 }
 
 // A call is cut over all its tiles at once: they stand in a row (sequence by sequence, in it head by head), `total` of them, and worker w of
-// `workers` (a wave, or a workgroup for 32-bit activations) has the tiles [first(w), first(w + 1)), whatever sequences they belong to.  So
+// `workers` (a wave, or a workgroup for 32-bit caches) has the tiles [first(w), first(w + 1)), whatever sequences they belong to.  So
 // sequences of unequal length load the card alike.  A piece (the part of one sequence and head that a worker has) leaves its state in slot
 // w + pair, pair = sequence * heads + head: along the row every piece has a larger w or a larger pair than the one before, so no two share one.
 OPS_FN int64_t attn_workers(int64_t total, int least, int most) {              // a worker has `least` tiles, if there are that many
@@ -52,22 +52,25 @@ enum { KV_U = 4 };
 OPS_FN int kv_parts(int kv_heads, int head_dim) { return (2 * kv_heads * head_dim + 512 * KV_U - 1) / (512 * KV_U); }
 
 struct AttnPlan { int heads, workers, least; size_t bytes; };
-enum { ATTN_MAX_SEQS = 1024, ATTN_WHOLE_TILES = 24 };      // sequences whose lengths a workgroup adds up; tiles that are not worth a cut
-// How a call is cut, from sizes alone.  `heads`: (key head, tile of query heads) pairs of a sequence; a workgroup each (workers 0) if the spans
-// are short, where joining would cost more than it gives, or the sequences so many that they fill the card.  Else the workers that the
-// card holds at a time share the tiles.
+enum { ATTN_MAX_SEQS = 1024 };      // sequences whose lengths a workgroup adds up
+// How a call is cut, from sizes alone.  `heads`: (key head, tile of query heads) pairs of a sequence.  A workgroup each (workers 0) if the spans are so
+// short that cutting and joining would cost more than it gives, or the sequences so many that they fill the card (2 query heads in bf16, us, whole /
+// cut: 16 pairs of 512 keys 10 / 12, of 768 13 / 12; 64 of 768 15 / 16, of 1024 18 / 17; 256 of 1024 22 / 29).  Else the workers that the card
+// holds at a time share the tiles.
 inline AttnPlan attention_plan(int dtype, bool coded, int head_dim, int kv_heads, int n_heads, int n_seqs, int max_len, int window) {
     AttnPlan p;
-    const bool f32 = dtype == 0;
-    const int group = n_heads / kv_heads, most = !f32 ? 16 : group < 3 ? group : 4;      // query heads of a pair
+    const bool rows = dtype == 0 && !coded;              // 32-bit caches: a kernel of their own
+    const int group = n_heads / kv_heads, most = !rows ? 16 : group < 3 ? group : 4;      // query heads of a pair
     const int64_t span = window > 0 && (int64_t)window + 31 < max_len ? (int64_t)window + 31 : max_len, tiles = (span + 31) / 32;
     p.heads = kv_heads * ((group + most - 1) / most);
-    p.least = f32 ? 8 : 1;
+    p.least = rows ? 8 : 1;
     p.workers = 0;
     p.bytes = 0;
-    if (tiles > ATTN_WHOLE_TILES && n_seqs <= ATTN_MAX_SEQS) {
-        const int64_t pairs = (int64_t)n_seqs * p.heads;
-        p.workers = (int)attn_workers(pairs * tiles, p.least, f32 ? 768 : coded ? 3072 : 2048);
+    const int64_t pairs = (int64_t)n_seqs * p.heads;
+    if (tiles > (pairs < 256 ? 24 : 32) && n_seqs <= ATTN_MAX_SEQS) {
+        // what the card holds, and no more pieces of a pair than the join is quick with (2 x 32768 tokens of one key head: 512 16 us, 1536 21)
+        const int64_t held = rows ? 768 : coded && (dtype != 0 || head_dim == 64) ? 3072 : 2048;
+        p.workers = (int)attn_workers(pairs * tiles, p.least, (int)(held < 512 * pairs ? held : 512 * pairs));
         // slots of up to `most` heads: (m, l) and the sums; then the row's length before each sequence
         p.bytes = (size_t)(p.workers + pairs) * (size_t)(group < most ? group : most) * (size_t)(head_dim + 2) * sizeof(float);
         p.bytes = (p.bytes + 15) / 16 * 16 + (size_t)(n_seqs + 1) * sizeof(int64_t);

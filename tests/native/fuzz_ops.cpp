@@ -41,8 +41,9 @@ static void cuts() {
     for (int it = 0; it < 3000; it++) {
         const int seqs = it % 4 ? pick(1, 12) : pick(1, 300), kv = pick(1, 8), group = pick(1, 20), dtype = pick(0, 2), hd = it % 2 ? 64 : 128;
         const int max_len = it % 7 ? pick(1, 40000) : pick(1, 400), window = it % 3 ? 0 : pick(1, 3000);
-        const AttnPlan p = attention_plan(dtype, it % 3 == 0, hd, kv, kv * group, seqs, max_len, window);
-        const int most = dtype ? 16 : group < 3 ? group : 4;
+        const bool coded = it % 3 == 0;
+        const AttnPlan p = attention_plan(dtype, coded, hd, kv, kv * group, seqs, max_len, window);
+        const int most = dtype || coded ? 16 : group < 3 ? group : 4;
         CHECK(p.heads == kv * ((group + most - 1) / most) && (p.bytes > 0) == (p.workers > 0));
         if (!p.workers) continue;
         std::vector<int64_t> before(seqs + 1, 0);
