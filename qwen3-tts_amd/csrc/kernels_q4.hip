@@ -446,7 +446,8 @@ template <int XT, int G, bool MINS> static hipError_t q4_rt(const Q4Args &a, hip
         return hipGetLastError();
     };
     const int64_t rows = (int64_t)a.n_out * ((a.n_rows + 15) / 16);              // the weights are gone through once for every 16 rows of x
-    if (rows <= 4096) return direct(1, q4_kernel<XT, G, MINS, 1>);
+    // few columns leave a workgroup few waves, which are slow to fetch many rows' scales (11954 x 128: 4.9 us, with 4 tiles 9.8; x 896: 8.9, 7.9)
+    if (rows <= 4096 || (slabs <= 4 && rows <= 16384)) return direct(1, q4_kernel<XT, G, MINS, 1>);
     if (rows <= 8192) return direct(2, q4_kernel<XT, G, MINS, 2>);
     if (rows <= 16384) return direct(4, q4_kernel<XT, G, MINS, 4>);
     // 16-bit rows of over 126 groups: the scales of 256 rows and x do not fit the LDS beside each other
