@@ -91,7 +91,6 @@ template <int T> __device__ __forceinline__ void store8(void *p, const float *f)
     }
 }
 
-template <int T> __device__ __forceinline__ float load1(const void *p, int64_t i) { return (float)((const typename Store<T>::type *)p)[i]; }
 template <int T> __device__ __forceinline__ void store1(void *p, int64_t i, float f) { ((typename Store<T>::type *)p)[i] = (typename Store<T>::type)f; }
 
 // The 8-bit types: scale = max|x| * (1 / TOP), both factors 32-bit numbers, code = x / scale (IEEE division, so the code is a function of
