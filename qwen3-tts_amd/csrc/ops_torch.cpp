@@ -115,7 +115,7 @@ const hipvoc_kv_cache *cache_of(const Call &c, PyObject *o) {
     const bool device = d && THPDevice_Check(d), here = device && ((THPDevice *)d)->device == c.device;
     Py_XDECREF(p);
     Py_XDECREF(d);
-    if (PyErr_Occurred()) throw Raised();
+    PyErr_Clear();
     if (!at || !device) refuse("cache must be a KvCache");
     if (!here) refuse("the cache is on another device than the handle, " + c.device.str());
     return (const hipvoc_kv_cache *)at;
@@ -209,6 +209,7 @@ PyObject *kv_read(const Call &c) {                     // cache, table, cu, firs
         v = {tv.data_ptr(), heads * hd, n, type};
     } else {
         if (!PyTuple_Check(c.arg[6]) || PyTuple_GET_SIZE(c.arg[6]) != 2) refuse("out must be a tuple of two tensors");
+        if (c.arg[5] != Py_None) refuse("dtype is out's where out is given");
         k = heads_of(c, PyTuple_GET_ITEM(c.arg[6], 0), heads, hd, "k");
         v = heads_of(c, PyTuple_GET_ITEM(c.arg[6], 1), heads, hd, "v");
         if (k.rows < n || v.rows < n || k.type != v.type) refuse("out must be two tensors of n_rows rows, alike in type");

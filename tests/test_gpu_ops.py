@@ -983,11 +983,40 @@ def test_refusals_of_shapes(pkg, ops):
     bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
     for bad in [lambda: ops.attention(bf(1, 4, 64), P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 12, 64), P.cache, P.table, P.lens_dev),
                 lambda: ops.attention(bf(64), P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 0, 64), P.cache, P.table, P.lens_dev),
+                lambda: ops.attention(None, P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 8, 64), None, P.table, P.lens_dev),
+                lambda: ops.attention(bf(1, 8, 64), P.cache, P.table, P.lens_dev, max_len=1 << 31), lambda: ops.attention(bf(1, 8, 64), P.cache, P.table, P.lens_dev, window=-1),
+                lambda: ops.attention(bf(1, 8, 64), P.cache, P.table, P.lens_dev.long()), lambda: ops.attention(bf(1, 8, 64), P.cache, P.table.cpu(), P.lens_dev),
+                lambda: ops.attention(bf(1, 8, 64).to_sparse(), P.cache, P.table, P.lens_dev), lambda: ops.attention(bf(1, 8, 64), P.cache, P.table, P.lens_dev, out=bf(2, 8, 64)),
+                lambda: ops.kv_read(P.cache, P.table, ints([0, 1]), ints([0]), 1, out=[bf(1, 8, 64)] * 2), lambda: ops.kv_read(P.cache, P.table, ints([0, 1]), ints([0]), -1),
+                lambda: ops.kv_read(P.cache, P.table, ints([0, 1]), ints([0]), 1, dtype="bf16"), lambda: ops.kv_read(P.cache, P.table, ints([0, 1]), ints([0]), 1, dtype=torch.int32),
+                lambda: ops.add_rmsnorm(bf(2, 8), bf(8), quant="int4"), lambda: ops.add_rmsnorm(bf(2, 8), bf(8), quant="int8", group=-32), lambda: ops.add_rmsnorm(bf(2, 8), bf(9)),
                 lambda: ops.add_rmsnorm(bf(1, 8).expand(1 << 22, 8).contiguous(), bf(8)), lambda: ops.add_rmsnorm(bf(1, 8).expand(4, 8), bf(8))]:
         with pytest.raises(pkg.HipVocError) as e:
             bad()
         assert e.value.code == -1 and len(str(e.value)) > 5
     ops.sync()
+
+
+def test_a_closed_handle_refuses(pkg):
+    o = pkg.HipOps.open(0)
+    o.close()
+    for call in (lambda: o.add_rmsnorm(torch.zeros((1, 8), device="cuda"), torch.zeros(8, device="cuda")), o.sync):
+        with pytest.raises(pkg.HipVocError):
+            call()
+    o.close()
+
+
+def test_outputs_keep_to_their_calls(ops):
+    """Results are tensors of their own: no call writes into what an earlier one gave, and what they hold is freed with them."""
+    x, w = rnd((64, 256), torch.float32, 1).cuda(), torch.ones(256, device="cuda")
+    first = ops.add_rmsnorm(x, w)[1]
+    kept = first.clone()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for i in range(200):
+        ops.add_rmsnorm(x + i, w, x)
+    torch.cuda.synchronize()
+    assert torch.equal(first, kept) and torch.cuda.memory_allocated() == before
 
 
 def test_calls_from_several_threads(pkg, ops):

@@ -4,7 +4,7 @@
 cd "$(dirname "$0")/../qwen3-tts_amd/csrc" || exit 1
 mkdir -p ../variants
 tag=$1; srcs=$2; flags=$3
-objs=" kernels.o kernels_bf16.o kernels_bf16_ring.o kernels_blk3.o kernels_enc.o kernels_gemm1.o kernels_wino.o scratch.o hipvoc.o safetensors.o wire.o discovery.o "
+objs=" kernels.o kernels_bf16.o kernels_bf16_ring.o kernels_blk3.o kernels_enc.o kernels_gemm1.o kernels_wino.o kernels_kv.o kernels_attn.o kernels_norm.o kernels_q4.o scratch.o hipvoc.o safetensors.o wire.o discovery.o "
 for src in ${srcs//,/ }; do
   base=${src%.*}
   extra=""; [ "$base" = kernels_wino ] && extra="-fno-slp-vectorize"
