@@ -2,8 +2,8 @@
 //
 // Mathematics: y[m][n] = sum_g s[n][g] * sum_{k in g} (c - 8) x[m][k], c = 0 .. 15 (with least values: s * c + min).  A code becomes a matrix
 // operand without any conversion: its four bits are put into the top of the mantissa of 16, so the operand is 16 + c exactly (bf16 has 7, f16 10
-// mantissa bits), and the group's sum is put right afterwards by (min - 16 s) or -24 s times X[m][g] = sum of x, which a matrix instruction with
-// ones gives in the same registers.  No product has a rounding; all sums are in 32 bits.  32-bit rows are cut into three bf16 parts of 8
+// mantissa bits), and the group's sum is put right afterwards by 16 (24 without least values) times X[m][g] = sum of x, which a matrix instruction
+// with ones gives in the same registers.  No product has a rounding; all sums are in 32 bits.  32-bit rows are cut into three bf16 parts of 8
 // mantissa bits each (exactly x together), three matrix instructions for one.  8-bit rows: a code's two's complement of (c - 8) is moved to the
 // top of a byte, 16 (c - 8), the group's sum is an exact integer, and 1/16 is part of the scale.
 // Bound: memory, half a byte per weight read once (non-temporal); next to it the vector ALU, which turns 8 codes into operands with 8 instructions
@@ -172,27 +172,44 @@ __device__ __forceinline__ void q4_use(const Q4Args &a, u32x4 (&w)[RT], X &&x, i
             constexpr unsigned ONE = F16 ? 0x3c003c00u : 0x3f803f80u;
             const u32x4 ones = {ONE, ONE, ONE, ONE};
             const unsigned e16 = Codes<XT>::sixteen();
+            // What the codes have too much comes off before the scale, so that the sum over groups never holds it; for 32-bit rows, whose result shows it,
+            // after every 32 columns (1536 columns in groups of 128: error 8.6e-7 -> 4.9e-7 of the result, 3 % of the time).
+            constexpr float EXTRA = MINS ? -16.f : -24.f;
+            constexpr bool OFTEN = XT == HIPVOC_T_F32;
             f32x4 acc[RT] = {}, sum = {};
 #pragma unroll
             for (int p = 0; p < PER; p++) {
                 const int c = g * PER + p;
                 u32x4 xc[XRow<XT>::P];
                 x(c, xc);
+                f32x4 here = OFTEN ? (f32x4){0.f, 0.f, 0.f, 0.f} : sum;
 #pragma unroll
-                for (int i = 0; i < XRow<XT>::P; i++) sum = mfma16(F16, xc[i], ones, sum);
+                for (int i = 0; i < XRow<XT>::P; i++) here = mfma16(F16, xc[i], ones, here);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
                     const u32x4 wc = Codes<XT>::of(w[t][c], e16);
+                    f32x4 v = OFTEN ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc[t];
 #pragma unroll
-                    for (int i = 0; i < XRow<XT>::P; i++) acc[t] = mfma16(F16, xc[i], wc, acc[t]);
+                    for (int i = 0; i < XRow<XT>::P; i++) v = mfma16(F16, xc[i], wc, v);
+                    if constexpr (OFTEN) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc[t][r] += fmaf(EXTRA, here[r], v[r]);
+                    } else {
+                        acc[t] = v;
+                    }
                 }
+                if constexpr (OFTEN) sum += here;
+                else sum = here;
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 const h16x2 p = sc[t * 16 * stride + g];
-                const float s = (float)p[0], off = MINS ? fmaf(-16.f, s, (float)p[1]) : -24.f * s;
+                const float s = (float)p[0], off = (float)p[1];
 #pragma unroll
-                for (int r = 0; r < 4; r++) out[t][r] = fmaf(s, acc[t][r], fmaf(off, sum[r], out[t][r]));
+                for (int r = 0; r < 4; r++) {
+                    out[t][r] = fmaf(s, OFTEN ? acc[t][r] : fmaf(EXTRA, sum[r], acc[t][r]), out[t][r]);
+                    if constexpr (MINS) out[t][r] = fmaf(off, sum[r], out[t][r]);
+                }
             }
         }
     };
