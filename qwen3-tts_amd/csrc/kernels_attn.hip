@@ -10,6 +10,8 @@
 // chunks gave the chip's dies unequal ones: 32 sequences of up to 4095 tokens, 8 key heads of 128, 16 query heads in bf16 (272 MB) 72 us, so 55.5 us
 // (4.9 TB/s).  131071 tokens, 32 query heads in f16 (537 MB) 96 us, 5.6 TB/s; 64 sequences of up to 8192 in 8 bits (566 MB) 110 us, 5.1 TB/s.
 // 32-bit activations, 32 sequences of up to 4095: 544 MB of 32-bit cache 109 us; 8 bits 51 us, alike for 1 to 8 query heads per key head.
+#include <type_traits>
+
 #include "ops_device.h"
 
 namespace hipvoc {
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     constexpr int LPR = HD / 8, KPS = 64 / LPR, U = 4, TILE = U * KPS, NW = 4;
     __shared__ float sh_o[NW][HT][HD], sh_m[NW][HT], sh_l[NW][HT];
     __shared__ int sh_bad[NW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = (lane % LPR) * 8, kl = lane / LPR;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = (lane % LPR) * 8, kl = lane / LPR;
     attn_pieces<HT>(a, [&](const AttnPiece &sp) {
         const int seq = sp.seq, kvh = sp.kvh, h0 = sp.h0, nh = min(HT, (kvh + 1) * a.group - h0);
         if (sp.bad && threadIdx.x == 0) raise(a.err, OPS_ERR_LENGTH);
@@ -172,13 +174,14 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         }
         const int32_t *table = a.table + seq * a.table_stride;
         bool bad = false;
-        for (int base = sp.from + wave * TILE; base < sp.to; base += NW * TILE) {
+        const auto tile = [&](int base, auto partial) {
+            constexpr bool PART = decltype(partial)::value;
             float k[U][8], v[U][8], s[HT][U];
             bool in[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int key = base + u * KPS + kl, kc = min(max(key, sp.lo), sp.to - 1);       // what is masked is read from a row that is not
-                in[u] = key >= sp.lo && key < sp.to;
+                const int key = base + u * KPS + kl, kc = PART ? min(max(key, sp.lo), sp.to - 1) : key;       // what is masked is read from a row that is not
+                in[u] = !PART || (key >= sp.lo && key < sp.to);
                 int page = table[kc >> a.page_shift];
                 if (!page_ok(page, a.c.n_pages)) { bad = true; page = 0; }
                 const int in_page = kc & (a.c.page - 1);
@@ -205,12 +208,20 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
                 for (int i = 0; i < 8; i++) o[h][i] *= old;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
+                    if (PART && h == 0) {                                // that row may hold an infinity, and 0 times it is NaN
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[u][i] = in[u] ? v[u][i] : 0.f;
+                    }
                     const float p = __builtin_amdgcn_exp2f(s[h][u] - safe);
                     l[h] += p;
 #pragma unroll
                     for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
                 }
             }
+        };
+        for (int base = sp.from + wave * TILE; base < sp.to; base += NW * TILE) {
+            if (base >= sp.lo && base + TILE <= sp.to) tile(base, std::false_type());
+            else tile(base, std::true_type());
         }
         const bool wave_bad = __any(bad);
         if (lane == 0) {
