@@ -69,8 +69,9 @@ inline AttnPlan attention_plan(int dtype, bool coded, int head_dim, int kv_heads
     const int64_t pairs = (int64_t)n_seqs * p.heads;
     if (tiles > (pairs < 256 ? 24 : 32) && n_seqs <= ATTN_MAX_SEQS) {
         // what the card holds, and no more pieces of a pair than the join is quick with (2 x 32768 tokens of one key head: 512 16 us, 1536 21)
-        // (3 workgroups a CU; 2 for 4 query heads with head_dim 128, 200 registers; else 12 or 8 waves)
-        const int64_t held = 256 * (rows ? (most == 4 && head_dim == 128 ? 2 : 3) : coded && (dtype != 0 || head_dim == 64) ? 12 : 8);
+        // (32-bit caches: 3 workgroups a CU, or 2 with the 200 registers of 4 query heads -- 3 x 6920 tokens, 28 heads on 4 of 64, planned for 2 / 3:
+        // 26 / 34 us; else 12 or 8 waves)
+        const int64_t held = 256 * (rows ? (most == 4 ? 2 : 3) : coded && (dtype != 0 || head_dim == 64) ? 12 : 8);
         p.workers = (int)attn_workers(pairs * tiles, p.least, (int)(held < 512 * pairs ? held : 512 * pairs));
         // slots of up to `most` heads: (m, l) and the sums; then the row's length before each sequence
         p.bytes = (size_t)(p.workers + pairs) * (size_t)(group < most ? group : most) * (size_t)(head_dim + 2) * sizeof(float);
