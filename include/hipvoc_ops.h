@@ -19,7 +19,9 @@
  *
  * Deferred errors: what only the device sees (a page number, a length or an offset out of range) is never followed out of
  * bounds.  The kernel records it in the handle, leaves such a row of the cache unwritten, fills such a row of an output
- * with NaN, and the next hipvoc_ops_sync / hipvoc_sync returns HIPVOC_E_CODE and clears the record.
+ * with NaN, and the next hipvoc_ops_sync / hipvoc_sync returns HIPVOC_E_CODE and clears the record.  The record is the handle's: a
+ * sync reports what any stream's calls raised until then, once.  A caller that has to tell streams or threads apart opens a handle
+ * for each (they hold 256 bytes of device memory).
  *
  * Types: "act" is the type of the step's own vectors, one of F32, F16, BF16.  Pointers to vectors are 16-byte aligned and
  * strides are counted in elements of their tensor.  Every sum, maximum, softmax statistic and scale is kept in 32 bits.
@@ -46,7 +48,8 @@ extern "C" {
  * encoder entry points refuse it. */
 void *hipvoc_ops_open(int device_id);
 
-/* Waits for `stream` (hipvoc_sync(h): for the whole device) and returns the deferred error, if any, clearing it. */
+/* Waits for `stream` (hipvoc_sync(h): for the whole device) and returns the handle's deferred error, if any, clearing it.  Callers that wait for
+ * different streams do not wait for each other. */
 int hipvoc_ops_sync(void *h, void *stream);
 
 /*

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <condition_variable>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -147,6 +148,9 @@ struct Ctx {
     bool trim_right = false;   // trans-conv trim policy (metadata transconv_trim_right_only=1): keep L*r samples instead of (L-1)*r
     bool is_encoder = false;   // handle made by hipvoc_enc_load (encoder.inc.cpp): the vocoder entry points refuse it
     bool is_ops = false;       // handle made by hipvoc_ops_open (ops.inc.cpp): no model; the vocoder and encoder entry points refuse it
+    std::mutex ops_words_lock;             // operator handles: which of the 64 words behind d_err are a collecting caller's (word 0: the error word)
+    std::condition_variable ops_word_free;
+    uint64_t ops_words = 1;
     bool bf16 = false;         // HIPVOC_DTYPE_BF16: conv-GEMM operands in bf16, fp32 accumulate, everything else fp32
     bool split3 = false;       // HIPVOC_DTYPE_BF16X3: bf16 = true as well; operands as two bf16 planes, three MFMAs per product
     int dual_out = 1;          // un-fused residual units, SnakeBeta in the producer's epilogue: 0 never, 1 conv7 -> conv1 only

@@ -152,9 +152,9 @@ static hipError_t kv_act(const KvMoveArgs &a, bool write, hipStream_t s) {
     return kv_st<HIPVOC_T_BF16>(a, write, s);
 }
 
-__global__ void take_error_kernel(int *err) { err[1] = atomicExch(err, 0); }
-hipError_t launch_take_error(int *err, hipStream_t s) {
-    take_error_kernel<<<1, 1, 0, s>>>(err);
+__global__ void take_error_kernel(int *err, int word) { err[word] = atomicExch(err, 0); }
+hipError_t launch_take_error(int *err, int word, hipStream_t s) {
+    take_error_kernel<<<1, 1, 0, s>>>(err, word);
     return hipGetLastError();
 }
 

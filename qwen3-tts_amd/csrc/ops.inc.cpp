@@ -19,8 +19,8 @@ struct DeviceScope {
     }
 };
 
-// Calls on one handle may come from several threads: what they share is the text of the last failure and the deferred error word.
-static std::mutex g_ops_sync;
+// Calls on one handle may come from several threads: what they share is the text of the last failure, the deferred error word and the words it is
+// collected in.
 static int ops_fail(Ctx *c, int code, const std::string &why) {
     std::lock_guard<std::mutex> lock(g_ops_text);
     c->err = why;
@@ -65,6 +65,26 @@ static int ops_move(Ctx *c, const char *what, bool write, const hipvoc_kv_cache 
     return ops_launched(c, what, write ? launch_kv_write(a, (hipStream_t)stream) : launch_kv_read(a, (hipStream_t)stream));
 }
 
+// One of the handle's words for a collecting caller, its own until the end: callers that wait for different streams do not wait for each other
+// (for one of 63 to end, if there are as many)
+struct OpsWord {
+    Ctx *c;
+    int word;
+    explicit OpsWord(Ctx *ctx) : c(ctx) {
+        std::unique_lock<std::mutex> lock(c->ops_words_lock);
+        c->ops_word_free.wait(lock, [this] { return ~c->ops_words != 0; });
+        word = __builtin_ctzll(~c->ops_words);
+        c->ops_words |= 1ull << word;
+    }
+    ~OpsWord() {
+        {
+            std::lock_guard<std::mutex> lock(c->ops_words_lock);
+            c->ops_words &= ~(1ull << word);
+        }
+        c->ops_word_free.notify_one();
+    }
+};
+
 // Takes the deferred error word on `stream` (one atomic exchange, so that nothing another stream raises meanwhile is lost) and waits for it.
 static int ops_collect(Ctx *c, hipStream_t stream) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -72,10 +92,10 @@ static int ops_collect(Ctx *c, hipStream_t stream) {
         return ops_fail(c, HIPVOC_E_ARG, "the stream is being captured: it cannot be waited for");
     int bits = 0;
     {
-        std::lock_guard<std::mutex> lock(g_ops_sync);      // d_err[1] is one caller's at a time
-        OPS_HIP(launch_take_error(c->d_err, stream));
+        const OpsWord mine(c);
+        OPS_HIP(launch_take_error(c->d_err, mine.word, stream));
         OPS_HIP(hipStreamSynchronize(stream));
-        OPS_HIP(hipMemcpyWithStream(&bits, c->d_err + 1, sizeof bits, hipMemcpyDeviceToHost, stream));
+        OPS_HIP(hipMemcpyWithStream(&bits, c->d_err + mine.word, sizeof bits, hipMemcpyDeviceToHost, stream));
     }
     if (!bits) return HIPVOC_OK;
     return ops_fail(c, HIPVOC_E_CODE, fmt("on the device:%s%s%s", bits & OPS_ERR_POSITION ? " a row's position outside its sequence's pages;" : "",
@@ -104,9 +124,9 @@ static void *ops_open_impl(int device_id) {
     c->device = device_id;
     c->is_ops = true;
     void *p = nullptr;
-    if (hipMalloc(&p, 256) != hipSuccess) return fail("hipMalloc failed");
+    if (hipMalloc(&p, 64 * sizeof(int)) != hipSuccess) return fail("hipMalloc failed");
     c->dev_allocs.push_back(p);
-    if (hipMemset(p, 0, 256) != hipSuccess || hipDeviceSynchronize() != hipSuccess) return fail("device error while opening");
+    if (hipMemset(p, 0, 64 * sizeof(int)) != hipSuccess || hipDeviceSynchronize() != hipSuccess) return fail("device error while opening");
     c->d_err = (int *)p;
     return c.release();
 }

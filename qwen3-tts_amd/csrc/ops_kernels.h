@@ -12,7 +12,7 @@ namespace hipvoc {
 // bits of the deferred error word of a handle
 enum OpsErr { OPS_ERR_POSITION = 1, OPS_ERR_PAGE = 2, OPS_ERR_LENGTH = 4 };
 
-hipError_t launch_take_error(int *err, hipStream_t s);      // err[1] = err[0], err[0] = 0
+hipError_t launch_take_error(int *err, int word, hipStream_t s);      // err[word] = err[0], err[0] = 0
 
 struct KvMoveArgs {
     hipvoc_kv_cache c;

@@ -156,7 +156,7 @@ class HipOps:
         return torch._C._cuda_getCurrentRawStream(self._index)
 
     def sync(self):
-        """Waits for the current stream and raises what the device found wrong since the last time."""
+        """Waits for the current stream and raises what the device found wrong since the last time, in calls of any stream on this handle."""
         rc = self._L.hipvoc_ops_sync(self._h, self.stream)
         if rc:
             raise HipVocError(rc, self._L.hipvoc_last_error(self._h).decode() if self._h else "the handle is closed")

@@ -35,3 +35,102 @@ def test_attention_of_an_infinity_in_a_32_bit_cache(ops, hd, kv, rep, lens, wind
             expect = want.clone()
             expect[b, head * rep:(head + 1) * rep, col] = -math.inf if i == 1 else math.inf
             assert torch.equal(out, expect) and torch.equal(got, lse), (b, t)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# several callers
+def test_syncs_do_not_wait_for_each_other(pkg, ops):  # noqa: F811
+    """While one thread waits for a stream that is busy, others that wait for idle ones return (a stream may stand behind the busy one in the same
+    hardware queue, so not all of six have to)."""
+    import threading
+    busy, done = torch.cuda.Stream(), torch.cuda.Event()
+    idle, handles = [torch.cuda.Stream() for _ in range(6)], [pkg.HipOps.open(0) for _ in range(3)] + [ops] * 3
+    for s, h in zip(idle, handles):                             # everything is loaded and warm
+        with torch.cuda.stream(s):
+            h.sync()
+    started, early = threading.Event(), []
+
+    def wait_for_busy():
+        with torch.cuda.stream(busy):
+            started.set()
+            ops.sync()
+
+    def wait_for_idle(s, h):
+        with torch.cuda.stream(s):
+            h.sync()
+            early.append(not done.query())
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(2_000_000_000)                        # about a second, then it ends
+        done.record()
+    first = threading.Thread(target=wait_for_busy)
+    first.start()
+    started.wait()
+    rest = [threading.Thread(target=wait_for_idle, args=(s, h)) for s, h in zip(idle, handles)]
+    threading.Event().wait(0.1)                                 # the first one is waiting by now
+    assert not done.query()
+    for t in rest:
+        t.start()
+    for t in rest + [first]:
+        t.join()
+    assert len(early) == 6 and any(early)
+    for h in handles[:3]:
+        h.close()
+
+
+def test_whose_errors_a_sync_reports(pkg, ops):  # noqa: F811
+    """One handle: the first sync behind the call reports it, whichever stream it waits for, and no other.  A handle each: the one whose call it was."""
+    P = Paged(ops, [40, 9], 1, 64, 8, "bf16", seed=3)
+    q = rnd((2, 2, 64), torch.bfloat16, 4).cuda()
+    bad = P.table.clone()
+    bad[0, 2] = P.cache.n_pages
+    torch.cuda.synchronize()
+    for one in (True, False):
+        mine, other = (ops, ops) if one else (ops, pkg.HipOps.open(0))
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        with torch.cuda.stream(streams[0]):
+            good = mine.attention(q, P.cache, P.table, P.lens_dev)
+        with torch.cuda.stream(streams[1]):
+            wrong = other.attention(q, P.cache, bad, P.lens_dev)
+        torch.cuda.synchronize()
+        raised = []
+        for s, h in zip(streams, (mine, other)):
+            with torch.cuda.stream(s):
+                try:
+                    h.sync()
+                    raised.append(False)
+                except pkg.HipVocError as e:
+                    raised.append(e.code == -2 and "page" in str(e))
+        assert raised == [one, not one]
+        assert bool(good.isfinite().all()) and bool(wrong[0].isnan().all()) and torch.equal(wrong[1], good[1])
+        ops.sync()
+        other.sync()
+        if not one:
+            other.close()
+
+
+def test_many_syncs_at_once(pkg, ops):  # noqa: F811
+    """More waiting threads than the handle has words: each gets one in its turn, and one error is reported once."""
+    import threading
+    P = Paged(ops, [40], 1, 64, 8, "bf16", seed=5)
+    q = rnd((1, 2, 64), torch.bfloat16, 4).cuda()
+    bad = P.table.clone()
+    bad[0, 2] = -3
+    ops.attention(q, P.cache, bad, P.lens_dev)
+    torch.cuda.synchronize()
+    seen, lock = [], threading.Lock()
+
+    def run():
+        for _ in range(20):
+            try:
+                ops.sync()
+                code = 0
+            except pkg.HipVocError as e:
+                code = e.code
+            with lock:
+                seen.append(code)
+    threads = [threading.Thread(target=run) for _ in range(100)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(seen) == 2000 and sorted(seen)[:2] == [-2, 0]
