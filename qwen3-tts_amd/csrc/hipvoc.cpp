@@ -1605,6 +1605,13 @@ static int decode_host_safe(Ctx *c, const void *codes, const int32_t *n_frames, 
     return rc;
 }
 
+// operator handles: calls may come from several threads, which share the text of the last failure
+static int ops_fail(Ctx *c, int code, const std::string &why) {
+    std::lock_guard<std::mutex> lock(g_ops_text);
+    c->err = why;
+    return code;
+}
+
 static void enc_release(Ctx *c);      // encoder.inc.cpp
 static int ops_sync_device(Ctx *c);   // ops.inc.cpp
 
@@ -1724,15 +1731,16 @@ void *hipvoc_load(const char *weights_path, int device_id, int dtype, int unit_f
     return nullptr;
 }
 
+// vocoder and encoder entry points: not on an operator handle, whose text has a lock and whose callers keep their current device
 #define CTX(h)                    \
     Ctx *c = (Ctx *)(h);          \
     if (!c) return HIPVOC_E_ARG;  \
+    if (c->is_ops) return ops_fail(c, HIPVOC_E_ARG, "this handle is an operator handle (hipvoc_ops_open)");  \
     if (hipSetDevice(c->device) != hipSuccess) { c->err = "hipSetDevice failed"; return HIPVOC_E_HIP; }
-// vocoder entry points: not on an encoder handle
+// vocoder entry points: not on an encoder handle either
 #define DEC(h)                    \
     CTX(h)                        \
-    if (c->is_encoder) { c->err = "this handle is an encoder (hipvoc_enc_load)"; return HIPVOC_E_ARG; }  \
-    if (c->is_ops) { c->err = "this handle is an operator handle (hipvoc_ops_open)"; return HIPVOC_E_ARG; }
+    if (c->is_encoder) { c->err = "this handle is an encoder (hipvoc_enc_load)"; return HIPVOC_E_ARG; }
 
 int hipvoc_max_tokens(void *h) { return h ? ((Ctx *)h)->unit_frames : HIPVOC_E_ARG; }
 int hipvoc_n_codebooks(void *h) { return h ? ((Ctx *)h)->n_q : HIPVOC_E_ARG; }

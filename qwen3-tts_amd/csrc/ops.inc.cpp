@@ -19,14 +19,6 @@ struct DeviceScope {
     }
 };
 
-// Calls on one handle may come from several threads: what they share is the text of the last failure, the deferred error word and the words it is
-// collected in.
-static int ops_fail(Ctx *c, int code, const std::string &why) {
-    std::lock_guard<std::mutex> lock(g_ops_text);
-    c->err = why;
-    return code;
-}
-
 #define OPS(h)                                                                                                             \
     Ctx *c = (Ctx *)(h);                                                                                                   \
     if (!c) return HIPVOC_E_ARG;                                                                                           \
@@ -65,7 +57,8 @@ static int ops_move(Ctx *c, const char *what, bool write, const hipvoc_kv_cache 
     return ops_launched(c, what, write ? launch_kv_write(a, (hipStream_t)stream) : launch_kv_read(a, (hipStream_t)stream));
 }
 
-// One of the handle's words for a collecting caller, its own until the end: callers that wait for different streams do not wait for each other
+// Calls on one handle may come from several threads, which share its deferred error word and the words it is collected in.
+// One of the latter for a collecting caller, its own until the end: callers that wait for different streams do not wait for each other
 // (for one of 63 to end, if there are as many)
 struct OpsWord {
     Ctx *c;

@@ -134,3 +134,39 @@ def test_many_syncs_at_once(pkg, ops):  # noqa: F811
     for t in threads:
         t.join()
     assert len(seen) == 2000 and sorted(seen)[:2] == [-2, 0]
+
+
+def test_texts_of_refusals_from_several_threads(pkg, ops):  # noqa: F811
+    """What the vocoder's and the encoder's entry points say to an operator handle is written like its own refusals: every text read is a whole one."""
+    import threading
+    L = ops._L
+    enc = pkg.encoder._lib()
+    other = "this handle is an operator handle (hipvoc_ops_open)"
+    assert L.hipvoc_decode(ops._h, None, 0, None, 0, None) == -1 and L.hipvoc_last_error(ops._h).decode() == other
+    assert L.hipvoc_ops_sync(ops._h, None) == 0
+    assert enc.hipvoc_enc_encode_batch(ops._h, None, None, 0, None, None, None) == -1 and L.hipvoc_last_error(ops._h).decode() == other
+    x, w = torch.zeros((2, 64), device="cuda"), torch.ones(64, device="cuda")
+    texts = {other, "eps must be finite and not negative", "group 7 must be 0, or for 8-bit rows 32, 64 or 128 and a divisor of cols 64"}
+    wrong = []
+
+    def run(i):
+        for _ in range(400):
+            if i % 3 == 0:
+                L.hipvoc_decode(ops._h, None, 0, None, 0, None)
+            elif i % 3 == 1:
+                enc.hipvoc_enc_encode_batch(ops._h, None, None, 0, None, None, None)
+            else:
+                try:
+                    ops.add_rmsnorm(x, w, **({"eps": -1.0} if i == 2 else {"group": 7}))
+                    wrong.append("not refused")
+                except pkg.HipVocError as e:
+                    if not any(t in str(e) for t in texts):
+                        wrong.append(str(e))
+            if L.hipvoc_last_error(ops._h).decode() not in texts:
+                wrong.append("text")
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
