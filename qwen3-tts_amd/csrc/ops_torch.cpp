@@ -7,6 +7,7 @@
 #include <torch/csrc/python_headers.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Device.h>
@@ -83,6 +84,8 @@ const at::Tensor &tensor(const Call &c, PyObject *o, const char *name) {
     const at::Tensor &t = THPVariable_Unpack(o);
     if (t.layout() != c10::kStrided) refuse(std::string(name) + " must be a strided tensor");
     if (t.device() != c.device) refuse(std::string(name) + " is on " + t.device().str() + ", the handle on " + c.device.str());
+    // a result without a graph would end the gradient without a word
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " requires grad, and the operators have no backward: call them under torch.no_grad() or on " + name + ".detach()");
     return t;
 }
 int type_of(c10::ScalarType t) {

@@ -4,6 +4,7 @@
 of it, so they can be captured into a graph with the rest of a step.  They allocate their results (and a workspace, where one
 is needed) as torch operations do; the C entry points take the caller's memory.  A refused call raises HipVocError before
 anything is launched; what only the device can see (a page number, a length) is raised by ``sync()``.
+They are for inference: there is no backward pass, and while gradients are recorded a tensor that requires one is refused.
 
 The tensors are looked at in _ops_torch.so (csrc/ops_torch.cpp), which calls the C entry points; here they have their names.
 There is NO fallback: if a shared library is missing or no HIP device is present, opening raises.
@@ -89,6 +90,9 @@ class KvCache:
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             _refuse("k and v must be [n_pages, kv_heads, page, head_dim], alike in shape, type and device")
         n, heads, page, hd = k.shape
+        for t in (k, v, k_scale, v_scale):
+            if t is not None and t.requires_grad:
+                _refuse("a cache's tensors carry no gradient: detach them")
         inner = (page * hd, hd, 1)
         stride = k.stride(0) if n > 1 else heads * page * hd
         if k.stride()[1:] != inner or v.stride()[1:] != inner or (n > 1 and v.stride(0) != stride):

@@ -170,3 +170,38 @@ def test_texts_of_refusals_from_several_threads(pkg, ops):  # noqa: F811
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# tensors that are more than their memory
+def test_gradients_are_refused_not_dropped(pkg, ops):  # noqa: F811
+    """There is no backward: a tensor that requires a gradient is refused while gradients are recorded, and taken under no_grad or inference_mode."""
+    P = Paged(ops, [9, 12], 2, 64, 8, "bf16", seed=1)
+    new, cu, first = rnd((2, 2, 64), torch.bfloat16, 1).cuda(), ints([0, 1, 2]), ints([8, 11])
+    q, x, w = rnd((2, 4, 64), torch.bfloat16, 1).cuda(), rnd((2, 64), torch.bfloat16, 2).cuda(), rnd((64,), torch.bfloat16, 3).cuda()
+    codes, scales = torch.randint(0, 256, (8, 32), dtype=torch.uint8, device="cuda"), torch.ones((8, 2), dtype=torch.float16, device="cuda")
+    grad = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    calls = {
+        "q": (lambda t: ops.attention(t, P.cache, P.table, P.lens_dev), q),
+        "out": (lambda t: ops.attention(q, P.cache, P.table, P.lens_dev, out=t), q),
+        "k": (lambda t: ops.kv_write(P.cache, t, new, P.table, cu, first), new),
+        "v": (lambda t: ops.kv_write(P.cache, new, t, P.table, cu, first), new),
+        "x": (lambda t: ops.add_rmsnorm(t, w, x), x),
+        "weight": (lambda t: ops.add_rmsnorm(x, t), w),
+        "residual": (lambda t: ops.add_rmsnorm(x, w, t), x),
+        "x ": (lambda t: ops.q4_matvec(codes, scales, t), x),
+        "scales": (lambda t: ops.q4_matvec(codes, t, x), scales),
+        "mins": (lambda t: ops.q4_matvec(codes, scales, x, mins=t), scales),
+    }
+    for name, (call, t) in calls.items():
+        leaf = grad(t)
+        for kind in (leaf, leaf * 1):
+            with pytest.raises(pkg.HipVocError) as e:
+                call(kind)
+            assert e.value.code == -1 and str(e.value).strip().split("requires grad")[0].endswith(name.strip() + " "), str(e.value)
+            with torch.no_grad():
+                call(kind)
+            with torch.inference_mode():
+                call(kind)
+            call(kind.detach())
+    ops.sync()

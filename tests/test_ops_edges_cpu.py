@@ -1,4 +1,4 @@
-"""How an attention is shared out, against what the compiled kernels let a CU hold."""
+"""How an attention is shared out, against what the compiled kernels let a CU hold; which tensors are no cache."""
 import os
 import re
 import shutil
@@ -55,3 +55,15 @@ def test_the_card_holds_the_workers_of_a_call_at_a_time(tmp_path):
                 assert workers <= 256 * 4 * held["attn_stream_kernel", (dtype, store, hd)], line
                 seen += 1
     assert seen == 2 * 20 * (1 + 2 + 2 * 3)
+
+
+def test_a_cache_is_memory_alone(pkg):
+    """A cache's tensors carry no gradient."""
+    import torch
+    ok, s = torch.zeros((3, 2, 16, 64)), torch.zeros((3, 2, 16))
+    q = torch.zeros((3, 2, 16, 64), dtype=torch.int8)
+    pkg.KvCache(ok, ok.clone())
+    for bad in [lambda: pkg.KvCache(ok.clone().requires_grad_(), ok), lambda: pkg.KvCache(ok, ok.clone().requires_grad_() * 2),
+                lambda: pkg.KvCache(q, q, s.clone().requires_grad_(), s)]:
+        with pytest.raises(pkg.HipVocError):
+            bad()
