@@ -86,6 +86,7 @@ const at::Tensor &tensor(const Call &c, PyObject *o, const char *name) {
     if (t.device() != c.device) refuse(std::string(name) + " is on " + t.device().str() + ", the handle on " + c.device.str());
     // a result without a graph would end the gradient without a word
     if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " requires grad, and the operators have no backward: call them under torch.no_grad() or on " + name + ".detach()");
+    if (t.is_neg()) refuse(std::string(name) + " is a view whose memory holds its negative: resolve_neg() makes it a tensor of its own");
     return t;
 }
 int type_of(c10::ScalarType t) {

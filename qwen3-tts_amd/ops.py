@@ -91,8 +91,8 @@ class KvCache:
             _refuse("k and v must be [n_pages, kv_heads, page, head_dim], alike in shape, type and device")
         n, heads, page, hd = k.shape
         for t in (k, v, k_scale, v_scale):
-            if t is not None and t.requires_grad:
-                _refuse("a cache's tensors carry no gradient: detach them")
+            if t is not None and (t.requires_grad or t.is_neg()):
+                _refuse("a cache's tensors carry no gradient (detach them) and are no views of a negative (resolve_neg)")
         inner = (page * hd, hd, 1)
         stride = k.stride(0) if n > 1 else heads * page * hd
         if k.stride()[1:] != inner or v.stride()[1:] != inner or (n > 1 and v.stride(0) != stride):

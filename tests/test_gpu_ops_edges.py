@@ -205,3 +205,16 @@ def test_gradients_are_refused_not_dropped(pkg, ops):  # noqa: F811
                 call(kind)
             call(kind.detach())
     ops.sync()
+
+
+def test_views_of_a_negative_are_refused(pkg, ops):  # noqa: F811
+    """The imaginary part of a conjugate is a real tensor whose memory holds its negative."""
+    z = torch.view_as_complex(rnd((2, 64, 2), torch.float32, 1).cuda()).conj().imag
+    assert z.is_neg() and z.dtype == torch.float32
+    flat = torch.empty_strided((2, 64), (64, 1), device="cuda")
+    neg = torch._neg_view(flat)
+    with pytest.raises(pkg.HipVocError) as e:
+        ops.add_rmsnorm(neg, torch.ones(64, device="cuda"))
+    assert e.value.code == -1 and "negative" in str(e.value)
+    ops.add_rmsnorm(neg.resolve_neg(), torch.ones(64, device="cuda"))
+    ops.sync()

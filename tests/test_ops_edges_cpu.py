@@ -58,12 +58,12 @@ def test_the_card_holds_the_workers_of_a_call_at_a_time(tmp_path):
 
 
 def test_a_cache_is_memory_alone(pkg):
-    """A cache's tensors carry no gradient."""
+    """A cache's tensors carry no gradient and are no views of a negative."""
     import torch
     ok, s = torch.zeros((3, 2, 16, 64)), torch.zeros((3, 2, 16))
     q = torch.zeros((3, 2, 16, 64), dtype=torch.int8)
     pkg.KvCache(ok, ok.clone())
-    for bad in [lambda: pkg.KvCache(ok.clone().requires_grad_(), ok), lambda: pkg.KvCache(ok, ok.clone().requires_grad_() * 2),
-                lambda: pkg.KvCache(q, q, s.clone().requires_grad_(), s)]:
+    for bad in [lambda: pkg.KvCache(ok.clone().requires_grad_(), ok), lambda: pkg.KvCache(ok, ok.clone().requires_grad_() * 2), lambda: pkg.KvCache(torch._neg_view(ok), ok),
+                lambda: pkg.KvCache(q, q, s.clone().requires_grad_(), s), lambda: pkg.KvCache(q, q, s, torch._neg_view(s))]:
         with pytest.raises(pkg.HipVocError):
             bad()
