@@ -70,7 +70,7 @@ typedef struct {
 /* The tokens of a call in the cache: a batch of n_seqs sequences, sequence b's rows being rows cu[b] .. cu[b+1]-1 of the
  * call's tensors and standing at its positions first[b], first[b]+1, ...; position p lives in page table[b*table_stride +
  * p/page], place p%page.  cu [n_seqs+1] is ascending and starts at 0 (rows at or behind cu[n_seqs] are padding: nothing is
- * read or written for them).  table_width: pages listed per sequence.  All int32, device memory. */
+ * written for them, and nothing that they hold is used; the call's tensors have n_rows rows, those among them).  table_width: pages listed per sequence.  All int32, device memory. */
 typedef struct {
     const int32_t *table, *cu, *first;
     int64_t table_stride;
