@@ -110,6 +110,7 @@ int hipvoc_attention(void *h, const hipvoc_kv_cache *cache, const void *q, int64
 
 /*
  * s = x + residual (in 32 bits; residual NULL: s = x), y = s / sqrt(mean(s^2) + eps) * weight, per row of `cols` values.
+ * eps may be 0: a row of zeros (or whose mean square is 0 in 32 bits) then has no norm, and its zeros give NaN (8 bits: scale NaN).
  * sum (act type; NULL: not wanted, and without a residual it has to be NULL) gets s rounded; y is made from s before that
  * rounding.  sum may be x or residual themselves (same stride); y overlaps no input and not sum.
  * out_dtype = dtype: y [rows][cols] in the act type.  INT8 / E4M3: y holds codes (bytes) and scales [rows][cols/group] f32,

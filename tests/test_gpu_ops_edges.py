@@ -218,3 +218,29 @@ def test_views_of_a_negative_are_refused(pkg, ops):  # noqa: F811
     assert e.value.code == -1 and "negative" in str(e.value)
     ops.add_rmsnorm(neg.resolve_neg(), torch.ones(64, device="cuda"))
     ops.sync()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# norm
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [5, 96, 640, 2056, 40000])
+def test_add_rmsnorm_with_eps_0(ops, act, cols):  # noqa: F811
+    """A row of zeros has no norm without eps: NaN, in 8 bits by its scale.  Its neighbours keep theirs."""
+    x = rnd((3, cols), ACT[act], cols).cuda()
+    w = (1 + 0.1 * rnd((cols,), torch.float32, 1)).to(ACT[act]).cuda()
+    x[1] = 0
+    zero = torch.zeros_like(x)
+    for res in (None, zero):
+        total, y = ops.add_rmsnorm(x, w, res, eps=0.0)
+        alone = ops.add_rmsnorm(x[::2].contiguous(), w, None, eps=0.0)[1]
+        assert bool(y[1].isnan().all()) and torch.equal(y[::2], alone) and bool(alone.isfinite().all())
+        assert res is None or torch.equal(total, x)
+        for quant in ("int8", "e4m3"):
+            for group in (0, 32):
+                if cols % (group or 1):
+                    continue
+                _, codes, scales = ops.add_rmsnorm(x, w, res, eps=0.0, quant=quant, group=group)
+                assert bool(scales[1].isnan().all()) and bool(scales[::2].isfinite().all()) and bool((codes[1].float() == 0).all())
+                back = codes.float().reshape(3, -1, group or cols) * scales[..., None]
+                assert bool(back[1].isnan().all()) and bool(back[::2].isfinite().all())
+    ops.sync()
