@@ -131,6 +131,7 @@ int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *res
  * Every product is exact; sums of a group, and of groups, are kept in 32 bits (8-bit rows: a group's sum is an integer).
  * Codes enter with 16 added that is taken off the sum, so a row of x that holds an infinity or NaN gives NaN, and one whose
  * sum of |x| * scale is within a factor of 31 of the largest 32-bit number may.
+ * Bits of a 32-bit x under 2^-133 count as 0 (values under 2^-109 lose accuracy).  y overlaps no input.
  * Any n_rows: the weights are read once for every 16.  x_stride is a multiple of 16 bytes.
  */
 int hipvoc_q4_matvec(void *h, const uint8_t *codes, const void *scales, const void *mins, int n_out, int n_in, int group,

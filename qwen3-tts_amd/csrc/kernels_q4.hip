@@ -76,7 +76,7 @@ template <int XT> struct XRow {
     }
     __device__ __forceinline__ void parts(u32x4 *p) const {
         if constexpr (XT == HIPVOC_T_F32) {
-            // x = a + b + c, each cut off (not rounded: nothing can overflow) after 8 significant bits
+            // x = a + b + c, each cut off (not rounded: nothing can overflow) after 8 significant bits, c not below bf16's least, 2^-133
             unsigned a[8], b[8], c[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {

@@ -244,3 +244,115 @@ def test_add_rmsnorm_with_eps_0(ops, act, cols):  # noqa: F811
                 back = codes.float().reshape(3, -1, group or cols) * scales[..., None]
                 assert bool(back[1].isnan().all()) and bool(back[::2].isfinite().all())
     ops.sync()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# 4-bit products
+Q4_SHAPES = [  # weight rows, group, groups, x rows: each kernel and tile count, whole slabs of 128 columns and not, at and over 128 groups
+    (17, 32, 1, 1), (33, 64, 3, 2), (100, 32, 129, 5), (70, 32, 257, 17), (300, 128, 130, 3), (4100, 64, 9, 3), (8190, 32, 131, 1), (8193, 32, 260, 2), (2050, 64, 17, 40),
+    (16390, 32, 33, 17), (16385, 32, 131, 5), (65541, 128, 3, 1), (65536, 32, 129, 2), (32769, 64, 5, 17), (65536, 64, 18, 16)]
+
+
+def whole_weights(n, group, groups, mins, seed, scales=(-1.0, -0.5, 0.25, 0.5, 1.0)):
+    """4-bit weights whose scales are powers of two and whose least values are quarters, and their values [n, k] in 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    draw = lambda high, shape, t: torch.randint(0, high, shape, generator=g, device="cuda", dtype=t)  # noqa: E731
+    codes = draw(256, (n, group * groups // 2), torch.uint8)
+    s = torch.tensor(scales, dtype=torch.float16, device="cuda")[draw(len(scales), (n, groups), torch.int64)]
+    least = ((draw(33, (n, groups), torch.int64) - 16).double() / 4).to(torch.float16) if mins else None
+    c = torch.stack((codes & 15, codes >> 4), -1).reshape(n, groups, group).double()
+    w = s.double()[..., None] * c + least.double()[..., None] if mins else s.double()[..., None] * (c - 8)
+    return codes, s, least, w.reshape(n, -1)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16", "int8"])
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("n,group,groups,m", Q4_SHAPES)
+def test_q4_products_of_whole_numbers(ops, act, mins, n, group, groups, m):  # noqa: F811
+    """x of whole numbers up to 2 and weights of quarters: every sum is a number of quarters under 2^24 in any order, so the result is exact before its
+    one rounding, and every column counts: x has something everywhere, in the last group alone, around the 128th group, in a single column."""
+    k = group * groups
+    assert 4 * k * 2 * (31 + 4) < 1 << 24                       # |x| <= 2, a code with 16 added <= 31, a least value <= 4, in quarters
+    codes, s, least, w = whole_weights(n, group, groups, mins, n + groups)
+    g = torch.Generator(device="cuda").manual_seed(m)
+    full = torch.randint(-2, 3, (m, k), generator=g, device="cuda").double()
+    parts = {"all": slice(0, k), "last": slice(k - group, k), "edge": slice(max(0, min(127 * group, k - 2 * group)), min(k, 129 * group)), "one": slice(k - 1, k)}
+    for where, at in parts.items():
+        x = torch.zeros_like(full)
+        x[:, at] = full[:, at] if where != "one" else full[:, at].abs() + 1
+        ref = torch.mm(x, w.t().contiguous())
+        if act == "int8":
+            for one in (True, False):                          # one scale for a row, or one for every group
+                xs = torch.full((m, 1 if one else groups), 0.5, device="cuda")
+                y = ops.q4_matvec(codes, s, x.to(torch.int8), mins=least, x_scale=xs)
+                assert torch.equal(y.double(), 0.5 * ref), (where, one)
+        else:
+            y = ops.q4_matvec(codes, s, x.to(ACT[act]), mins=least)
+            assert torch.equal(y, ref.float().to(ACT[act])), where
+    ops.sync()
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("n,group,groups,m", Q4_SHAPES)
+def test_q4_products_keep_all_of_a_32_bit_x(ops, mins, n, group, groups, m):  # noqa: F811
+    """x has three columns of 1 + 2^-10 + 2^-18, one for each of the bf16 that carry it.  A code with 16 added makes that 23 bits, the sum of three with least
+    values under 2^6 has 24: exact in any order (but where all three meet in one block), and without the last part off by 2^-18 of a weight."""
+    k = group * groups
+    codes, s, least, w = whole_weights(n, group, groups, mins, n, scales=(-1.0, 1.0))
+    least = None if least is None else least.round()
+    if mins:
+        c = torch.stack((codes & 15, codes >> 4), -1).reshape(n, groups, group).double()
+        w = (s.double()[..., None] * c + least.double()[..., None]).reshape(n, k)
+    value = 1 + 2.0 ** -10 + 2.0 ** -18
+    x = torch.zeros((m, k), dtype=torch.float64, device="cuda")
+    for i in range(m):
+        for at in {(3 + 5 * i) % k, k // 2, k - 1 - i % group}:
+            x[i, at] = value if i % 2 else -value
+    assert bool((x.float().double() == x).all())
+    ref = torch.mm(x, w.t().contiguous())
+    y = ops.q4_matvec(codes, s, x.float(), mins=least)
+    ops.sync()
+    # two columns in one block of 32 give codes with 16 added up to 2 * 31 * value < 2^6, 24 bits; all three in one, where there is but one block, up to
+    # 3 * 31 * value < 2^7, so each of the nine additions there, the step that takes 24 off and the two into the sums may round by half of 2^-17
+    assert float((y.double() - ref).abs().max()) <= (12 * 2.0 ** -18 if k == 32 else 0)
+
+
+@pytest.mark.parametrize("n,group,groups,m", [(33, 64, 3, 2), (100, 32, 129, 5), (70, 32, 257, 17), (8193, 32, 260, 2), (65536, 32, 129, 2), (16390, 32, 33, 17)])
+@pytest.mark.parametrize("mins", [False, True])
+def test_q4_error_of_32_bit_rows(ops, mins, n, group, groups, m):  # noqa: F811
+    """The root mean square of the error where roundings are independent.  Of a scale's worth, x of spread 1: a block of 32 columns has up to 3 x 32 additions
+    (two such blocks, with codes and with ones) whose partial sums are up to 31 sqrt(32) (times 24 for the ones) / 24, so sqrt(2 * 3 k) * 31 * sqrt(32);
+    the k / 32 blocks and 2 k / group steps of the sums over them have partial sums of up to (8 + |least| / |scale|) sqrt(k).  Each rounding is under 2^-24 of its partial sum."""
+    k = group * groups
+    codes, s, least, w = whole_weights(n, group, groups, mins, groups, scales=(-1.0, 1.0))
+    x = rnd((m, k), torch.float32, 5).cuda()
+    ref = torch.mm(x.double(), w.t().contiguous())
+    y = ops.q4_matvec(codes, s, x, mins=least)
+    ops.sync()
+    rms = float((y.double() - ref).square().mean().sqrt())
+    bound = 2.0 ** -24 * (math.sqrt(6 * k) * 31 * math.sqrt(32) + math.sqrt(k / 32 + 2 * k / group) * (16 + 4) * math.sqrt(k) + float(ref.square().mean().sqrt()))
+    assert rms <= bound, rms / bound
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_q4_products_of_small_numbers(ops, act):  # noqa: F811
+    """x around the least normal number of its type, subnormal ones among them, bit for bit; of 32-bit ones bits under 2^-133 are lost, no more."""
+    codes, s, least, w = whole_weights(50, 32, 9, False, 3, scales=(-1.0, 1.0))
+    step = {"f32": 2.0 ** -133, "f16": 2.0 ** -24, "bf16": 2.0 ** -133}[act]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for big in (3, 100):
+        x = torch.randint(-big, big + 1, (4, 288), generator=g, device="cuda").double() * step
+        assert bool((x.to(ACT[act]).double() == x).all())
+        ref = torch.mm(x, w.t().contiguous())
+        y = ops.q4_matvec(codes, s, x.to(ACT[act]))
+        ops.sync()
+        assert torch.equal(y, ref.float().to(ACT[act])), big
+    if act == "f32":
+        for e in (-104, -112, -118, -124, -130):
+            x = (rnd((4, 288), torch.float32, 7) * 2.0 ** e).cuda()
+            ref = torch.mm(x.double(), w.t().contiguous())
+            y = ops.q4_matvec(codes, s, x)
+            ops.sync()
+            # cut off below 2^-133, times a weight of up to 8; the rest as in any product (31 for a code with 16 added, 24 off again: 55)
+            bound = 288 * 8 * 2.0 ** -133 + (288 + 16) * 2.0 ** -24 * 55 * x.double().abs().sum(-1, keepdim=True) + 2.0 ** -149
+            assert bool(((y.double() - ref).abs() <= bound).all()), e
