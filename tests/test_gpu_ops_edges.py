@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops import ACT, Paged, ints, ops, rnd  # noqa: F401
+from test_gpu_ops import ACT, U32, Layer, Paged, ints, ops, rnd, u  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -356,3 +356,55 @@ def test_q4_products_of_small_numbers(ops, act):  # noqa: F811
             # cut off below 2^-133, times a weight of up to 8; the rest as in any product (31 for a code with 16 added, 24 off again: 55)
             bound = 288 * 8 * 2.0 ** -133 + (288 + 16) * 2.0 ** -24 * 55 * x.double().abs().sum(-1, keepdim=True) + 2.0 ** -149
             assert bool(((y.double() - ref).abs() <= bound).all()), e
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the operators together
+class Recorded(Layer):
+    """A layer whose products are all kept: `out` name -> (rows, their scales, result)."""
+
+    def project(self, ops, name, x, x_scale=None):  # noqa: F811
+        y = super().project(ops, name, x, x_scale)
+        self.out[name] = (x, x_scale, y)
+        return y
+
+
+def check_residual_norm(x, r, w, total, codes, scales, eps, group):
+    """bf16 rows to int8, as check_norm bounds them: the sum is one rounding, y has cols / 2 + 12 in 32 bits, a code half a step."""
+    s = x.double() + r.double()
+    assert bool(((total.double() - s).abs() <= (u(torch.bfloat16) + 2 * U32) * s.abs()).all())
+    cols = x.shape[1]
+    y = (s / torch.sqrt((s * s).mean(-1, keepdim=True) + eps) * w.double()).reshape(x.shape[0], -1, group)
+    rel = (cols / 2 + 12) * U32
+    top, sc = y.abs().amax(-1), scales.double()
+    assert bool(((sc - top / 127).abs() <= (rel + 4 * U32) * top / 127).all())
+    back = codes.double().reshape(y.shape) * sc[..., None]
+    assert bool(((back - y).abs() <= (rel * y.abs() + sc[..., None] * (0.5 + 127 * 4 * U32)) * (1 + 1e-6)).all())
+
+
+@pytest.mark.parametrize("store", ["same", "e4m3"])
+def test_every_stage_of_a_layer(ops, store):  # noqa: F811
+    """All four products and both norms of a layer's token steps against 64 bits on the stage's own inputs."""
+    lay, B = Recorded(seed=5), 3
+    lay.out = {}
+    P = Paged(ops, [0, 7, 29], lay.kv, lay.hd, 8, "bf16", store, seed=3, extra_pages=24, width=8)
+    used = set(P.table[P.table >= 0].tolist())
+    free = iter([p for p in range(P.cache.n_pages) if p not in used])
+    table = torch.tensor([[p if p >= 0 else next(free) for p in row] for row in P.table.tolist()], dtype=torch.int32, device="cuda")
+    x, res = rnd((B, 256), torch.bfloat16, 1).cuda(), rnd((B, 256), torch.bfloat16, 2).cuda()
+    for t in range(6):
+        lens, keep = [n + t + 1 for n in P.lens], {}
+        d, h2 = lay.step(ops, x, res, P.cache, table, ints(lens), ints([0, 1, 2, 3]), ints([n - 1 for n in lens]), 64, keep)
+        ops.sync()
+        kk = {n: v.cpu() for n, v in keep.items()}
+        check_residual_norm(x.cpu(), res.cpu(), lay.norm[0], kk["h"], kk["c"], kk["s"], 1e-5, 32)
+        check_residual_norm(kk["o"], kk["h"], lay.norm[1], kk["h2"], kk["c2"], kk["s2"], 1e-5, 32)
+        assert set(lay.out) == {"qkv", "o", "up", "down"}
+        for name, (xin, sc, y) in lay.out.items():
+            _, _, least, w, s = lay.w[name]
+            xv = xin.cpu().double() if sc is None else xin.cpu().double() * sc.cpu().double().repeat_interleave(32, 1)
+            ref = xv @ w.t()
+            mag = xv.abs() @ (55 * s).t() + (xv.abs() @ least.double().abs().repeat_interleave(32, 1).t() if least is not None else 0)
+            assert bool(((y.cpu().double() - ref).abs() <= 1.01 * (mag * (xv.shape[1] + 16) * U32 + u(torch.bfloat16) * ref.abs())).all()), name
+        assert torch.equal(kk["f"], torch.nn.functional.silu(lay.out["up"][2]).cpu())
+        x, res = d, h2
