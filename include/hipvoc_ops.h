@@ -15,7 +15,8 @@
  * device; they are read and written when the stream gets there.  No call allocates, synchronises (but for hipvoc_ops_sync /
  * hipvoc_sync) or changes the calling thread's current device, so all of them can be captured into a HIP graph (which must
  * not outlive the handle: the kernels report into it); every kernel writes all it reads back, so two graphs share nothing
- * that they are not given both.  A call whose threads do not count in 32 bits is refused.
+ * that they are not given both.  A call whose threads do not count in 32 bits is refused, and so are more than 2^28 rows of a
+ * cache call, 65535 sequences, 1024 key heads, 16384 query heads, 2^24 rows of weights or 2^20 columns.
  *
  * Deferred errors: what only the device sees (a page number, a length or an offset out of range) is never followed out of
  * bounds.  The kernel records it in the handle, leaves such a row of the cache unwritten, fills such a row of an output
@@ -94,7 +95,8 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
  * them) and query head i reading key head i / (n_heads / kv_heads),
  *   out[b][i] = sum_t p_t v_t,   p = softmax_t(scale * q[b][i] . k_t),   lse[b][i] = log sum_t exp(scale * q . k_t)
  * over the positions max(0, n - window) <= t < n (window 0: all).  n = 0: out is 0 and lse -infinity.
- * q, out: act type, row b at b*q_stride / b*out_stride, [n_heads][head_dim]; lse [n_seqs][n_heads] f32 or NULL.
+ * q, out: act type, row b at b*q_stride / b*out_stride, [n_heads][head_dim]; lse [n_seqs][n_heads] f32 or NULL.  out may be q
+ * itself (same stride); else it overlaps no input.
  * max_len: no lens[b] is larger (a larger one is a deferred error); the host cuts the length into parts by it, so a
  * tight bound costs least.  At most table_width * page.
  * Where act has 16 bits the weights p enter the product with V as the sum of two f16 (an f16 cache) or two bf16 (any other), so an
@@ -132,7 +134,7 @@ int hipvoc_add_rmsnorm(void *h, const void *x, int64_t x_stride, const void *res
  * Codes enter with 16 added that is taken off the sum, so a row of x that holds an infinity or NaN gives NaN, and one whose
  * sum of |x| * scale is within a factor of 31 of the largest 32-bit number may.
  * Bits of a 32-bit x under 2^-133 count as 0 (values under 2^-109 lose accuracy).  y overlaps no input.
- * Any n_rows: the weights are read once for every 16.  x_stride is a multiple of 16 bytes.
+ * Up to 65535 rows: the weights are read once for every 16.  x_stride is a multiple of 16 bytes.
  */
 int hipvoc_q4_matvec(void *h, const uint8_t *codes, const void *scales, const void *mins, int n_out, int n_in, int group,
                      const void *x, int64_t x_stride, int x_dtype, const float *x_scale, int x_groups, void *y,
