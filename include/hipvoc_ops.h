@@ -100,7 +100,7 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
  * max_len: no lens[b] is larger (a larger one is a deferred error); the host cuts the length into parts by it, so a
  * tight bound costs least.  At most table_width * page.
  * Where act has 16 bits the weights p enter the product with V as the sum of two f16 (an f16 cache) or two bf16 (any other), so an
- * infinity among the values that are seen gives NaN; scores, sums and the product itself are in 32 bits.
+ * infinity among the values that are seen gives NaN (in an F32 cache it stays one); scores, sums and the product itself are in 32 bits.
  * How a sequence is cut, and with it the order of its sums, depends on all lengths of the call; the same call gives the same bits.
  * workspace: hipvoc_attention_workspace() bytes (it may be 0), 16-byte aligned, not used by another call in flight.
  */

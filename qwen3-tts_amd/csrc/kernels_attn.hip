@@ -9,7 +9,8 @@
 // joined by a second kernel, without atomics: the order of every sum follows from the call's lengths.  A grid of fixed
 // chunks gave the chip's dies unequal ones: 32 sequences of up to 4095 tokens, 8 key heads of 128, 16 query heads in bf16 (272 MB) 72 us, so 55.5 us
 // (4.9 TB/s).  131071 tokens, 32 query heads in f16 (537 MB) 96 us, 5.6 TB/s; 64 sequences of up to 8192 in 8 bits (566 MB) 110 us, 5.1 TB/s.
-// 32-bit activations, 32 sequences of up to 4095: 544 MB of 32-bit cache 109 us; 8 bits 51 us, alike for 1 to 8 query heads per key head.
+// 32-bit activations, 32 sequences of up to 4095: 544 MB of 32-bit cache 109 us; 8 bits as fast as 16-bit activations (below).  32-bit caches, 4 query heads
+// at a time: 3 x 6920 tokens, 28 heads on 4 of 64 (read twice): 26 us, 16 heads 22.
 #include <type_traits>
 
 #include "ops_device.h"
@@ -262,8 +263,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 //                 turns them with one byte permutation per two values; row m of product i is column m HD/16 + i.
 // So neither K, V nor P passes through LDS.  Scores, m, l and O are in 32 bits; P goes into the product with V as two values of V's own type (bf16 for
 // 8-bit codes, which bf16 and f16 hold exactly, and whose scales are in the scores and in P): see weights().  A 32-bit q or weight is three bf16, exactly:
-// three matrix instructions for one, still under the time of an 8-bit row's loads (the vector ALU's rate bound 32-bit activations on 8-bit caches by its
-// conversions and, for over 4 query heads per key head, a second reading).
+// three matrix instructions for one, which cost no time: 32 sequences of 2048 .. 4095 tokens, 8 key heads of 128 in INT8 (203 MB), 16 query heads 50 us in
+// 32 bits and 52 in bf16, 64 query heads 55 and 58.
 // What is masked is read from a row that is not (so that no stale value, NaN or page number behind the last token matters).
 
 // four codes to two pairs of 16-bit values, exactly

@@ -24,6 +24,7 @@ OPS_EXPORTS = [
 T_F32, T_F16, T_BF16, T_INT8, T_E4M3 = 0, 1, 2, 3, 4      # include/hipvoc_ops.h: HIPVOC_T_*
 
 
+# The C entry points for a caller that holds addresses, not tensors: their structs, and in _lib() their arguments.
 class _Cache(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("page_stride", C.c_int64),
                 ("n_pages", C.c_int32), ("kv_heads", C.c_int32), ("page", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
@@ -83,7 +84,7 @@ def _type(t) -> int:
 
 class KvCache:
     """Names the tensors of a paged cache (hipvoc_kv_cache): k, v [n_pages, kv_heads, page, head_dim], contiguous within a page;
-    k_scale, v_scale [n_pages, kv_heads, page] float32 for int8 / float8_e4m3fn caches."""
+    k_scale, v_scale [n_pages, kv_heads, page] float32 for int8 / float8_e4m3fn caches.  None of them requires a gradient."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _bind_torch()
