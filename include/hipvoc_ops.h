@@ -49,8 +49,8 @@ extern "C" {
  * encoder entry points refuse it. */
 void *hipvoc_ops_open(int device_id);
 
-/* Waits for `stream` (hipvoc_sync(h): for the whole device) and returns the handle's deferred error, if any, clearing it.  Callers that wait for
- * different streams do not wait for each other. */
+/* Waits for `stream` (hipvoc_sync(h): for the whole device) and returns the handle's deferred error, if any, clearing it.  Callers
+ * that wait for different streams do not wait for each other. */
 int hipvoc_ops_sync(void *h, void *stream);
 
 /*
@@ -71,7 +71,8 @@ typedef struct {
 /* The tokens of a call in the cache: a batch of n_seqs sequences, sequence b's rows being rows cu[b] .. cu[b+1]-1 of the
  * call's tensors and standing at its positions first[b], first[b]+1, ...; position p lives in page table[b*table_stride +
  * p/page], place p%page.  cu [n_seqs+1] is ascending and starts at 0 (rows at or behind cu[n_seqs] are padding: nothing is
- * written for them, and nothing that they hold is used; the call's tensors have n_rows rows, those among them).  table_width: pages listed per sequence.  All int32, device memory. */
+ * written for them, and nothing that they hold is used; the call's tensors have n_rows rows, those among them).  table_width:
+ * pages listed per sequence.  All int32, device memory. */
 typedef struct {
     const int32_t *table, *cu, *first;
     int64_t table_stride;
@@ -100,7 +101,8 @@ int hipvoc_kv_read(void *h, const hipvoc_kv_cache *cache, void *k, void *v, int6
  * max_len: no lens[b] is larger (a larger one is a deferred error); the host cuts the length into parts by it, so a
  * tight bound costs least.  At most table_width * page.
  * Where act has 16 bits the weights p enter the product with V as the sum of two f16 (an f16 cache) or two bf16 (any other), so an
- * infinity among the values that are seen gives NaN (in an F32 cache it stays one); scores, sums and the product itself are in 32 bits.
+ * infinity among the values that are seen gives NaN (in an F32 cache it stays one); scores, sums and the product itself are in
+ * 32 bits.
  * How a sequence is cut, and with it the order of its sums, depends on all lengths of the call; the same call gives the same bits.
  * workspace: hipvoc_attention_workspace() bytes (it may be 0), 16-byte aligned, not used by another call in flight.
  */
