@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -15,6 +16,15 @@ GOLDEN = os.path.join(ROOT, "tests", "golden")
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run by the driver with -m gpu)")
+
+
+@pytest.fixture(autouse=True)
+def _no_garbage_where_memory_is_counted(request):
+    """What earlier tests left in reference cycles (a caught error holds its frames, and they their tensors) is freed before a test that compares
+    torch's allocated bytes, not somewhere inside it."""
+    code = getattr(request.function, "__code__", None)
+    if code is not None and "memory_allocated" in code.co_names:
+        gc.collect()
 
 
 @pytest.fixture(scope="session")
